@@ -63,6 +63,14 @@ int wpc_attention_plain(const void* q, int q_stride, void* out, int out_stride, 
                         const int* positions, int T, int nh, int nkv, int hd, float scale, int window,
                         int n_splits, float* part, cudaStream_t stream);
 
+// sinks: the first positions that a query sees beside its window (0 without a window);
+// lse: null, or [T][nh] for each row's maximum + log2(sum) of its scores in units of log 2
+int wpc_attention_plain_bounded(const void* q, int q_stride, void* out, int out_stride, int dtype,
+                                const void* k_pages, const void* v_pages, const int* page_table, int table_width,
+                                const int* seq_of_token, const int* positions, int T, int nh, int nkv, int hd,
+                                float scale, int window, int sinks, int n_splits, float* part, float* lse,
+                                cudaStream_t stream);
+
 int wpc_attention_mma_supports(int nh, int nkv, int hd);
 int wpc_attention_decode_early_pages(int on);
 int wpc_attention_decode(const void* q, int q_stride, void* out, int out_stride, const void* k_pages,
@@ -85,6 +93,51 @@ int wpc_attention_prefill_tc(const void* q, int q_stride, void* out, int out_str
                              const void* v_pages, const int* page_table, int table_width, const int* cu_seqlens,
                              const int* ctx_lens, int B, int max_new, int nh, int nkv, int hd, float scale,
                              int window, int* status, int n_pages, int tiles, cudaStream_t stream);
+
+int wpc_attention_prefill_tc_bounded(const void* q, int q_stride, void* out, int out_stride, const void* k_pages,
+                                     const void* v_pages, const int* page_table, int table_width,
+                                     const int* cu_seqlens, const int* ctx_lens, int B, int max_new, int nh, int nkv,
+                                     int hd, float scale, int window, int sinks, float* lse, int* status, int n_pages,
+                                     cudaStream_t stream);
+
+// Attention with sinks beside a window (sinks > 0, window > 0), or over all earlier positions with what
+// the sums of weights need (window = 0, sinks = 0, scores, row_ml / lse given): attention_bounded.cu.
+// decode: cluster 0: n_ctas CTAs share all pages (part_o, part_ml, counters as in
+// wpc_attention_decode); else `groups` clusters of that size to a pair (as in
+// wpc_attention_decode_cluster).  scores: float32 [B * nkv][nh / nkv][score_stride], score_stride a
+// multiple of 64 that covers the longest context; row_ml: float32 [B][nh][2].
+int wpc_attention_decode_bounded(const void* q, int q_stride, void* out, int out_stride, const void* k_pages,
+                                 const void* v_pages, const int* page_table, int table_width, const int* ctx_lens,
+                                 int B, int nh, int nkv, int hd, float scale, int window, int sinks, int n_ctas,
+                                 int cluster, int groups, float* part_o, float* part_ml, int* counters, int n_counters,
+                                 float* scores, int score_stride, float* row_ml, cudaStream_t stream);
+int wpc_attention_prefill_bounded(const void* q, int q_stride, void* out, int out_stride, const void* k_pages,
+                                  const void* v_pages, const int* page_table, int table_width, const int* cu_seqlens,
+                                  const int* ctx_lens, int B, int max_new, int nh, int nkv, int hd, float scale,
+                                  int window, int sinks, float* lse, cudaStream_t stream);
+
+// attention_sums.cu: the weight that each cached entry received, added to weight_sums
+// [n_pages][nkv][64] (an entry of the step's own tokens begins with it, and its place in
+// stored_positions gets its token's position).  decode: from what wpc_attention_decode_bounded
+// left; plain: from q, k and the rows' log-sums.
+int wpc_weight_sums_decode(const float* scores, int score_stride, const float* row_ml, const int* page_table,
+                           int table_width, const int* ctx_lens, const int* token_positions, int B, int nh, int nkv,
+                           int max_ctx, int n_pages, float* weight_sums, int* stored_positions, int* status,
+                           cudaStream_t stream);
+int wpc_weight_sums_plain(const void* q, int q_stride, int dtype, const void* k_pages, const int* page_table,
+                          int table_width, const int* cu_seqlens, const int* ctx_lens, const int* token_positions,
+                          const float* lse, int B, int nh, int nkv, int hd, float scale, int max_ctx, int n_pages,
+                          float* weight_sums, int* stored_positions, int* status, cudaStream_t stream);
+
+// eviction.cu.  kept: int32 [layers][B][nkv][keep], the entry that belongs at each place of the kept
+// part (-1 behind a shorter sequence).  weight_sums, stored_positions: [layers][n_pages][nkv][64].
+int wpc_select_kept(const float* weight_sums, const int* stored_positions, const int* page_table, int table_width,
+                    const int* lens, const int* next_positions, int layers, int B, int nkv, int n_pages,
+                    int keep, int sinks, int recent, int* kept, int* status, cudaStream_t stream);
+// k_bytes, v_bytes: bytes of an entry's key and value
+int wpc_move_kept(void* k_pages, void* v_pages, int k_bytes, int v_bytes, float* weight_sums, int* stored_positions,
+                  const int* page_table, int table_width, const int* kept, int layers, int B, int nkv, int n_pages,
+                  int keep, int* status, cudaStream_t stream);
 
 int wpc_sample(const float* logits, int n_rows, int V, const int* slots, long long* seq_state, float temperature,
                const int* banned, int n_banned, int* out, cudaStream_t stream);

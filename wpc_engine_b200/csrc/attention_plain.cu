@@ -4,6 +4,10 @@
 // kernels (wpc-runtime/src/model.rs:476-510).  When the queries are few and their contexts
 // long (a decode step of the 32-bit path), the keys of a query are divided evenly among
 // several blocks, whose partial results a second kernel adds up in order.
+// A query sees the keys first .. its own and, with `sinks`, the first `sinks` keys beside them: its
+// list of keys is the sinks before `first`, then the rest.  `lse`, if given, gets each row's
+// maximum + log2(sum) of the scores in units of log 2 (for the sums of weights,
+// attention_sums.cu).
 #include "api.h"
 #include "common.cuh"
 
@@ -26,7 +30,8 @@ attention_plain_kernel(const T* __restrict__ q, int q_stride, T* __restrict__ ou
                        const T* __restrict__ k_pages, const T* __restrict__ v_pages,
                        const int* __restrict__ page_table, int table_width,
                        const int* __restrict__ seq_of_token, const int* __restrict__ positions,
-                       int nh, int nkv, int hd, float scale, int window, float* __restrict__ part) {
+                       int nh, int nkv, int hd, float scale, int window, int sinks, float* __restrict__ lse,
+                       float* __restrict__ part) {
   pdl_trigger();
   pdl_wait();
   extern __shared__ float smem[];
@@ -40,9 +45,12 @@ attention_plain_kernel(const T* __restrict__ q, int q_stride, T* __restrict__ ou
   const int* table = page_table + (size_t)b * table_width;
   // this block's share of the keys that the query sees (all of them with one block to a query)
   const int first = (window > 0 && pos - window + 1 > 0) ? pos - window + 1 : 0;
-  const int n_splits = gridDim.z, per = (pos - first + 1 + n_splits - 1) / n_splits;
-  const int lo = first + (int)blockIdx.z * per;
-  const int n_keys = max(min(pos + 1, lo + per) - lo, 0);
+  const int ns = min(sinks, first);           // sinks before the window: number j < ns of the list is key j,
+  const int all = ns + pos - first + 1;       // a later one is key first + j - ns
+  const int n_splits = gridDim.z, per = (all + n_splits - 1) / n_splits;
+  const int lo = (int)blockIdx.z * per;
+  const int n_keys = max(min(all, lo + per) - lo, 0);
+  const int skipped = first - ns;
 
   const T* qrow = q + (size_t)t * q_stride + (size_t)h * hd;
   for (int d = threadIdx.x; d < hd; d += AP_THREADS) qs[d] = to_float(qrow[d]);
@@ -55,8 +63,8 @@ attention_plain_kernel(const T* __restrict__ q, int q_stride, T* __restrict__ ou
     const int cn = min(AP_CHUNK, n_keys - c0);
     float m_loc = -INFINITY;
     for (int j = threadIdx.x; j < cn; j += AP_THREADS) {
-      const int p = lo + c0 + j;
-      const int page = table[p / WPC_PAGE];
+      const int p = lo + c0 + j + (lo + c0 + j < ns ? 0 : skipped);
+      const int page = max(table[p / WPC_PAGE], 0);
       const T* kr = k_pages + (((size_t)page * nkv + kvh) * WPC_PAGE + p % WPC_PAGE) * hd;
       float dot = 0.f;
       if ((hd & 3) == 0) {                              // the same order of additions, four elements a load
@@ -92,9 +100,10 @@ attention_plain_kernel(const T* __restrict__ q, int q_stride, T* __restrict__ ou
       if (d < hd) {
         float a = acc[u] * corr;
         for (int j = 0; j < cn;) {                       // page by page: one look-up for up to 64 keys
-          const int p = lo + c0 + j;
-          const int in_page = p % WPC_PAGE, n = min(cn - j, WPC_PAGE - in_page);
-          const T* vr = v_pages + (((size_t)table[p / WPC_PAGE] * nkv + kvh) * WPC_PAGE + in_page) * hd + d;
+          const int at = lo + c0 + j, p = at + (at < ns ? 0 : skipped);
+          const int in_page = p % WPC_PAGE;
+          const int n = min(at < ns ? min(cn - j, ns - at) : cn - j, WPC_PAGE - in_page);
+          const T* vr = v_pages + (((size_t)max(table[p / WPC_PAGE], 0) * nkv + kvh) * WPC_PAGE + in_page) * hd + d;
           for (int i = 0; i < n; ++i) a = fmaf(ps[j + i], to_float(vr[(size_t)i * hd]), a);
           j += n;
         }
@@ -117,6 +126,7 @@ attention_plain_kernel(const T* __restrict__ q, int q_stride, T* __restrict__ ou
     }
     return;
   }
+  if (lse && threadIdx.x == 0) lse[(size_t)t * nh + h] = m_run * 1.4426950408889634f + log2f(l_run);
   T* orow = out + (size_t)t * out_stride + (size_t)h * hd;
   const float inv = l_run > 0.f ? 1.0f / l_run : 0.f;
 #pragma unroll
@@ -129,13 +139,21 @@ attention_plain_kernel(const T* __restrict__ q, int q_stride, T* __restrict__ ou
 // Adds up the partial results of a query's blocks, in block order.
 template <typename T>
 __global__ void attention_plain_combine_kernel(const float* __restrict__ part, T* __restrict__ out, int out_stride, int nh,
-                                               int hd, int n_splits) {
+                                               int hd, int n_splits, float* __restrict__ lse) {
   pdl_trigger();
   pdl_wait();
   const int t = blockIdx.x, h = blockIdx.y;
   const float* prow = part + ((size_t)t * nh + h) * n_splits * (hd + 2);
   float m = -INFINITY;
   for (int z = 0; z < n_splits; ++z) m = fmaxf(m, prow[(size_t)z * (hd + 2) + hd]);
+  if (lse && threadIdx.x == 0) {
+    float den = 0.f;
+    for (int z = 0; z < n_splits; ++z) {
+      const float* pz = prow + (size_t)z * (hd + 2);
+      den = fmaf(pz[hd] == -INFINITY ? 0.f : expf(pz[hd] - m), pz[hd + 1], den);
+    }
+    lse[(size_t)t * nh + h] = m * 1.4426950408889634f + log2f(den);
+  }
   for (int d = threadIdx.x; d < hd; d += blockDim.x) {
     float num = 0.f, den = 0.f;
     for (int z = 0; z < n_splits; ++z) {
@@ -157,21 +175,31 @@ extern "C" int wpc_attention_plain(const void* q, int q_stride, void* out, int o
                                    int table_width, const int* seq_of_token, const int* positions, int T, int nh,
                                    int nkv, int hd, float scale, int window, int n_splits, float* part,
                                    cudaStream_t stream) {
+  return wpc_attention_plain_bounded(q, q_stride, out, out_stride, dtype, k_pages, v_pages, page_table, table_width,
+                                     seq_of_token, positions, T, nh, nkv, hd, scale, window, 0, n_splits, part, nullptr,
+                                     stream);
+}
+
+extern "C" int wpc_attention_plain_bounded(const void* q, int q_stride, void* out, int out_stride, int dtype,
+                                           const void* k_pages, const void* v_pages, const int* page_table,
+                                           int table_width, const int* seq_of_token, const int* positions, int T,
+                                           int nh, int nkv, int hd, float scale, int window, int sinks, int n_splits,
+                                           float* part, float* lse, cudaStream_t stream) {
   // n_splits > 1: that many blocks share the keys of each query; part: float32 scratch of
   // T * nh * n_splits * (hd + 2) elements for their partial results
   if (T <= 0) return 0;
   if (hd < 1 || hd > 2 * AP_THREADS || nkv < 1 || nh % nkv) return WPC_ERR_UNSUPPORTED;
-  if (n_splits < 1 || n_splits > 65535 || (n_splits > 1 && !part)) return WPC_ERR_BAD_ARGUMENT;
+  if (n_splits < 1 || n_splits > 65535 || (n_splits > 1 && !part) || sinks < 0) return WPC_ERR_BAD_ARGUMENT;
   const size_t smem = (size_t)(hd + AP_CHUNK) * sizeof(float);
   dim3 grid(T, nh, n_splits);
   WPC_DISPATCH_DTYPE(dtype, Tt,
                      wpc::launch(attention_plain_kernel<Tt>, grid, AP_THREADS, smem, stream, 
                          (const Tt*)q, q_stride, (Tt*)out, out_stride, (const Tt*)k_pages, (const Tt*)v_pages,
-                         page_table, table_width, seq_of_token, positions, nh, nkv, hd, scale, window, part));
+                         page_table, table_width, seq_of_token, positions, nh, nkv, hd, scale, window, sinks, lse, part));
   int rc = launch_status();
   if (rc || n_splits == 1) return rc;
   WPC_DISPATCH_DTYPE(dtype, Tt,
                      wpc::launch(attention_plain_combine_kernel<Tt>, dim3(T, nh), 128, 0, stream, (const float*)part,
-                                 (Tt*)out, out_stride, nh, hd, n_splits));
+                                 (Tt*)out, out_stride, nh, hd, n_splits, lse));
   return launch_status();
 }

@@ -206,13 +206,18 @@ __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map
       : "memory");
 }
 
-template <int HD, int NT>
+// SINKS: beside its window a query sees the first `sinks` positions.  Their pages that lie before
+// the window's first page come first; pages are counted in one range (see attention_mma.cuh).
+// lse, if given, gets each row's maximum + log2(sum) in units of log 2, for the sums of weights
+// (attention_sums.cu).
+template <int HD, int NT, bool SINKS>
 __global__ void __launch_bounds__(WsCfg<HD, NT>::THREADS, NT == 2 ? 1 : 2)
 prefill_ws_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                   const __nv_bfloat16* __restrict__ q, int q_stride, __nv_bfloat16* __restrict__ out, int out_stride,
                   const int* __restrict__ page_table, int table_width, const int* __restrict__ cu_seqlens,
                   const int* __restrict__ ctx_lens, int nh, int nkv, float scale_log2, int window,
-                  int* __restrict__ status, unsigned long long wait_ns, int starve, int n_sm, int late_trigger) {
+                  int* __restrict__ status, unsigned long long wait_ns, int starve, int n_sm, int late_trigger,
+                  int sinks, float* __restrict__ lse) {
   using C = Cfg<HD>;
   using W = WsCfg<HD, NT>;
   constexpr int NS = W::NS;
@@ -287,8 +292,10 @@ prefill_ws_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
   const int tile_pos_hi = start + last_row / n_rep;
   const int tile_pos_lo = start + row0 / n_rep;
   const int tile_lo = (window > 0 && tile_pos_lo - window + 1 > 0) ? tile_pos_lo - window + 1 : 0;
-  const int blk0 = tile_lo / PAGE, blk1 = tile_pos_hi / PAGE + 1;
+  const int first = tile_lo / PAGE, ns = SINKS ? min((sinks + PAGE - 1) / PAGE, first) : 0;
+  const int blk0 = first - ns, blk1 = tile_pos_hi / PAGE + 1;
   const int n_pg = blk1 - blk0;
+  auto block = [&](int j) { return SINKS && j < ns ? j : blk0 + j; };   // page j of the CTA's list
 
   fence_before_sync();
   __syncthreads();
@@ -303,11 +310,11 @@ prefill_ws_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     if (lane == 0 && !starve) {
       asm volatile("prefetch.tensormap [%0];" ::"l"(&map_k) : "memory");
       asm volatile("prefetch.tensormap [%0];" ::"l"(&map_v) : "memory");
-      int page_next = max(table[blk0], 0);
+      int page_next = max(table[block(0)], 0);
       for (int j = 0; j < n_pg; ++j) {
         const int st = j % NS, n = j / NS;
         const int row = (page_next * nkv + g) * PAGE;
-        if (j + 1 < n_pg) page_next = max(table[blk0 + j + 1], 0);
+        if (j + 1 < n_pg) page_next = max(table[block(j + 1)], 0);
         if (!mbar_wait(k_empty + st, (n & 1) ^ 1, wait_ns)) { atomicExch(failed, 1); break; }
         mbar_expect_tx(k_full + st, C::PAGE_BYTES);
 #pragma unroll
@@ -410,11 +417,11 @@ prefill_ws_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
       tmem_ld_wait();
       fence_before_sync();
       mbar_arrive(s_empty + t * 2 + bb);                   // the score buffer may be overwritten
-      const int abs0 = (blk0 + j) * PAGE;
+      const int abs0 = block(j) * PAGE;
       // four partial maxima (and sums below): a single running value would be a chain of 64
       // dependent instructions.  Only pages that this row does not see whole are masked.
       float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-      if (valid && abs0 + PAGE - 1 <= p_row && abs0 >= lo_row) {
+      if (valid && abs0 + PAGE - 1 <= p_row && (abs0 >= lo_row || (SINKS && abs0 + PAGE <= sinks))) {
 #pragma unroll
         for (int i = 0; i < 64; i += 8) {                  // (pairs of values to a maximum: one three-input instruction)
           mx4[0] = fmaxf(fmaxf(mx4[0], __uint_as_float(su[i])), __uint_as_float(su[i + 1]));
@@ -426,7 +433,7 @@ prefill_ws_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
 #pragma unroll
         for (int i = 0; i < 64; ++i) {
           const int kabs = abs0 + i;
-          const float sc = (valid && kabs >= lo_row && kabs <= p_row) ? __uint_as_float(su[i]) : -INFINITY;
+          const float sc = (valid && (kabs >= lo_row || (SINKS && kabs < sinks)) && kabs <= p_row) ? __uint_as_float(su[i]) : -INFINITY;
           su[i] = __float_as_uint(sc);
           mx4[i & 3] = fmaxf(mx4[i & 3], sc);
         }
@@ -484,6 +491,18 @@ prefill_ws_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
       // are issued after this page's P V and run after it.
       tmem_st32(tmem_S(t, bb) + lane_off, pw);
       tmem_st_wait();
+      if ((SINKS || lse) && abs0 + PAGE > L) {
+        // behind the end of the sequence lies what the page's last owner left: a weight of zero
+        // times an infinity would be no zero, so those value rows are cleared before P V
+        ok = mbar_wait(v_full + j % NS, (j / NS) & 1, wait_ns);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        uint8_t* v_page = base + NT * C::Q_BYTES + (NS + j % NS) * C::PAGE_BYTES;
+        for (int e = rt + (L - abs0) * 8; e < PAGE * 8; e += ROWS)
+#pragma unroll
+          for (int hb = 0; hb < C::NB; ++hb) *(uint4*)(v_page + hb * (PAGE * 128) + e * 16) = make_uint4(0, 0, 0, 0);
+        fence_async_smem();
+      }
       fence_before_sync();
       mbar_arrive(p_full + t);
     }
@@ -495,6 +514,7 @@ prefill_ws_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     if (!ok) atomicExch(failed, 1);
     if (ok) {
       const float inv = l_sum > 0.f ? 1.f / l_sum : 0.f;
+      if (lse && valid) lse[(size_t)(tok0 + t_row) * nh + h_row] = m_used + log2f(l_sum);
       __nv_bfloat16* dst = out + (size_t)(tok0 + t_row) * out_stride + (size_t)h_row * HD;
 #pragma unroll
       for (int c = 0; c < HD; c += 32) {
@@ -531,13 +551,14 @@ prefill_ws_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
   }
 }
 
-template <int HD, int NT>
+template <int HD, int NT, bool SINKS = false>
 static int launch_ws(const void* q, int q_stride, void* out, int out_stride, const void* k_pages, const void* v_pages,
                      int n_pages, const int* page_table, int table_width, const int* cu_seqlens, const int* ctx_lens,
-                     int B, int max_new, int nh, int nkv, float scale, int window, int* status, cudaStream_t stream) {
+                     int B, int max_new, int nh, int nkv, float scale, int window, int* status, cudaStream_t stream,
+                     int sinks = 0, float* lse = nullptr) {
   using W = WsCfg<HD, NT>;
   static int configured[MAX_DEVICES];
-  if (int rc = allow_smem(prefill_ws_kernel<HD, NT>, W::SMEM, configured)) return rc;
+  if (int rc = allow_smem(prefill_ws_kernel<HD, NT, SINKS>, W::SMEM, configured)) return rc;
   // the cache as a matrix [n_pages * nkv * PAGE, HD]: a page of one KV head is 64 of its rows
   const long rows = (long)n_pages * nkv * PAGE;
   if (rows > 0x7fffffffL) return WPC_ERR_TOO_LARGE;
@@ -548,10 +569,10 @@ static int launch_ws(const void* q, int q_stride, void* out, int out_stride, con
   if (rc) return rc;
   const int n_rep = nh / nkv;
   dim3 grid(nkv, (max_new * n_rep + NT * ROWS - 1) / (NT * ROWS), B);
-  wpc::launch(prefill_ws_kernel<HD, NT>, grid, W::THREADS, W::SMEM, stream, mk, mv, (const __nv_bfloat16*)q, q_stride,
+  wpc::launch(prefill_ws_kernel<HD, NT, SINKS>, grid, W::THREADS, W::SMEM, stream, mk, mv, (const __nv_bfloat16*)q, q_stride,
               (__nv_bfloat16*)out, out_stride, page_table, table_width, cu_seqlens, ctx_lens, nh, nkv, scale * LOG2E,
               window, status, wait_policy().limit_ns, wait_policy().starve, NT == 1 ? sm_count() : 1 << 30,
-              max_new >= 1024 ? 1 : 0);
+              max_new >= 1024 ? 1 : 0, sinks, lse);
   return launch_status();
 }
 
@@ -588,6 +609,29 @@ int wpc_attention_prefill_tc(const void* q, int q_stride, void* out, int out_str
 #undef WPC_WS
   }
   return WPC_ERR_BAD_ARGUMENT;
+}
+
+// The same with sinks beside a window, and, where lse is given (no window, no sinks), each row's
+// maximum + log2(sum) into lse [T][nh].  One row tile to a CTA.
+int wpc_attention_prefill_tc_bounded(const void* q, int q_stride, void* out, int out_stride, const void* k_pages,
+                                     const void* v_pages, const int* page_table, int table_width,
+                                     const int* cu_seqlens, const int* ctx_lens, int B, int max_new, int nh, int nkv,
+                                     int hd, float scale, int window, int sinks, float* lse, int* status, int n_pages,
+                                     cudaStream_t stream) {
+  if (B <= 0 || max_new <= 0) return 0;
+  if (!wpc_attention_prefill_tc_supports(nh, nkv, hd) || (q_stride % 8) || (out_stride % 8) ||
+      (((uintptr_t)q | (uintptr_t)out | (uintptr_t)k_pages | (uintptr_t)v_pages) & 15))
+    return WPC_ERR_UNSUPPORTED;
+  if (sinks < 0 || (sinks > 0 && window <= 0)) return WPC_ERR_BAD_ARGUMENT;
+#define WPC_WS(HD_, SINKS_)                                                                                          \
+  return wpc::fatc::launch_ws<HD_, 1, SINKS_>(q, q_stride, out, out_stride, k_pages, v_pages, n_pages, page_table,  \
+                                              table_width, cu_seqlens, ctx_lens, B, max_new, nh, nkv, scale, window, \
+                                              status, stream, sinks, lse)
+  if (hd == 128 && sinks) WPC_WS(128, true);
+  if (hd == 128) WPC_WS(128, false);
+  if (sinks) WPC_WS(64, true);
+  WPC_WS(64, false);
+#undef WPC_WS
 }
 
 }  // extern "C"

@@ -9,6 +9,7 @@ torch does on this path.
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 import threading
 from typing import Optional, Tuple
@@ -628,7 +629,9 @@ def attention(q: torch.Tensor, n_heads: int, n_kv_heads: int, head_dim: int, k_p
               v_pages: torch.Tensor, page_table: torch.Tensor, cu_seqlens: torch.Tensor, ctx_lens: torch.Tensor,
               seq_of_token: torch.Tensor, positions: torch.Tensor, scale: float, window: Optional[int],
               max_new_tokens: int, max_ctx_len: int, splits: Optional[int] = None,
-              mma_only: bool = False, cluster: Optional[int] = None, groups: int = 1) -> torch.Tensor:
+              mma_only: bool = False, cluster: Optional[int] = None, groups: int = 1, sinks: int = 0,
+              weight_sums: Optional[torch.Tensor] = None, stored_positions: Optional[torch.Tensor] = None,
+              token_positions: Optional[torch.Tensor] = None) -> torch.Tensor:
     """softmax(q . k * scale) . v over the cached positions that each query sees: 0..its own,
     or the last `window` of them.  q: the first n_heads*head_dim columns of each row.
 
@@ -636,7 +639,29 @@ def attention(q: torch.Tensor, n_heads: int, n_kv_heads: int, head_dim: int, k_p
     split-KV kernel when every sequence brings one token (csrc/attention_mma.cu; `splits` forces
     about that many CTAs to a pair, `cluster` `groups` clusters of that size to a pair, 0 none); otherwise the
     tcgen05 kernel for head sizes 64 and 128 (csrc/attention_tc.cu) and the mma.sync kernel for
-    the others (or with `mma_only`).  Everything else runs the plain kernel."""
+    the others (or with `mma_only`).  Everything else runs the plain kernel.
+
+    `sinks`: beside its window a query sees the first `sinks` positions (their pages must be in the
+    page table; pages between the sinks and the window may be gone).  Without a window it
+    changes nothing.
+
+    `weight_sums` (float32 [n_pages, n_kv_heads, PAGE], no window): the weight that every cached
+    entry receives from the step's queries, summed over queries and the heads of a KV head's
+    group, is added to the entry's place there; the entries of the step's own tokens begin with
+    it, and their places in `stored_positions` (int32, the same shape) get `token_positions[t]`
+    (int32 [T]).  `positions` are places in the cache here, `token_positions` those in the text:
+    they differ once entries have been taken out (`select_kept`).  No page may belong to two
+    sequences of the step."""
+    if weight_sums is not None or stored_positions is not None or token_positions is not None:
+        return _attention_with_sums(q, n_heads, n_kv_heads, head_dim, k_pages, v_pages, page_table, cu_seqlens, ctx_lens,
+                                    seq_of_token, positions, scale, window, max_new_tokens, max_ctx_len, splits,
+                                    mma_only, cluster, groups, sinks, weight_sums, stored_positions, token_positions)
+    if sinks:
+        _need(sinks > 0, f"sinks must not be negative, got {sinks}")
+        if window:
+            return _attention_with_sinks(q, n_heads, n_kv_heads, head_dim, k_pages, v_pages, page_table, cu_seqlens,
+                                         ctx_lens, seq_of_token, positions, scale, window, max_new_tokens, max_ctx_len,
+                                         splits, mma_only, cluster, groups, sinks)
     if q.dtype != torch.bfloat16 or not library().wpc_attention_mma_supports(n_heads, n_kv_heads, head_dim):
         return attention_plain(q, n_heads, n_kv_heads, head_dim, k_pages, v_pages, page_table, seq_of_token,
                                positions, scale, window, max_ctx_len)
@@ -687,6 +712,220 @@ def attention(q: torch.Tensor, n_heads: int, n_kv_heads: int, head_dim: int, k_p
             page_table.shape[1], _p(cu_seqlens), _p(ctx_lens), B, max_new_tokens, n_heads, n_kv_heads, head_dim,
             ctypes.c_float(scale), int(window or 0), _stream()))
     return out
+
+
+def _check_step(q, n_heads, n_kv_heads, head_dim, k_pages, v_pages, page_table, cu_seqlens, ctx_lens, seq_of_token,
+                positions) -> None:
+    """The arguments that all attention of a step over the paged cache shares."""
+    _rows(q, "q")
+    dev, T, B = q.device, q.shape[0], ctx_lens.numel()
+    _need(dev.index == torch.cuda.current_device(),
+          f"the tensors lie on {dev}, but the current device is cuda:{torch.cuda.current_device()}")
+    _need(n_kv_heads >= 1 and n_heads % n_kv_heads == 0, "n_heads must be a multiple of n_kv_heads")
+    _need(q.shape[1] >= n_heads * head_dim, "q is too narrow")
+    shape = (n_kv_heads, PAGE, head_dim)
+    _need(k_pages.dim() == 4 and k_pages.shape == v_pages.shape and tuple(k_pages.shape[1:]) == shape
+          and k_pages.is_contiguous() and v_pages.is_contiguous() and k_pages.dtype == q.dtype == v_pages.dtype
+          and k_pages.device == dev and v_pages.device == dev,
+          "pages must be contiguous [n_pages, n_kv_heads, PAGE, head_dim] of q's type, on its device")
+    _need(page_table.dim() == 2 and page_table.shape[0] == B, "page_table must have a row for every sequence")
+    for name, t, n in (("page_table", page_table, page_table.numel()), ("cu_seqlens", cu_seqlens, B + 1),
+                       ("ctx_lens", ctx_lens, B), ("seq_of_token", seq_of_token, T), ("positions", positions, T)):
+        _need(t.dtype == torch.int32 and t.is_contiguous() and t.numel() == n and t.device == dev,
+              f"{name} must be contiguous int32 of {n} elements on {dev}")
+
+
+def _decode_scratch(n_seqs, n_kv_heads, n_heads, head_dim, n_ctas, cluster, groups, device):
+    """(part_o, part_ml, tickets) of a decode step's split work, for this call alone: calls on other
+    streams and captured graphs share nothing.  None where no two CTAs share a pair through memory."""
+    pairs = n_seqs * n_kv_heads
+    if cluster:
+        if groups == 1:
+            return None, None, None
+        n_o, n_ml = pairs * groups * (n_heads // n_kv_heads) * head_dim, pairs * groups * 32
+    else:
+        slots = n_ctas + pairs
+        n_o, n_ml = slots * 16 * head_dim, slots * 16 * 2
+    part = torch.empty((n_o + n_ml,), dtype=torch.float32, device=device)
+    return part, part[n_o:], torch.zeros((pairs,), dtype=torch.int32, device=device)
+
+
+@functools.lru_cache(maxsize=4096)
+def _bounded_decode_plan(n_seqs, n_kv_heads, n_heads, head_dim, blocks, splits, cluster, groups, n_sms):
+    """(cluster, groups, n_ctas) of a decode step in which a query sees `blocks` pages."""
+    ctx = blocks * PAGE
+    if cluster is None:
+        cluster, groups = (0, 1) if splits else plan_decode_cluster(n_seqs, n_kv_heads, n_heads, head_dim, ctx, None)
+    return cluster, groups, 0 if cluster else plan_decode_ctas(n_seqs, n_kv_heads, ctx, None, splits)
+
+
+def _attention_with_sinks(q, n_heads, n_kv_heads, head_dim, k_pages, v_pages, page_table, cu_seqlens, ctx_lens,
+                          seq_of_token, positions, scale, window, max_new_tokens, max_ctx_len, splits, mma_only,
+                          cluster, groups, sinks) -> torch.Tensor:
+    _need(window > 0, f"window must be positive, got {window}")
+    _check_step(q, n_heads, n_kv_heads, head_dim, k_pages, v_pages, page_table, cu_seqlens, ctx_lens, seq_of_token, positions)
+    sinks, window = min(int(sinks), 1 << 30), min(int(window), 1 << 30)
+    T, B, dev = q.shape[0], ctx_lens.numel(), q.device
+    lib = library()
+    if q.dtype != torch.bfloat16 or not lib.wpc_attention_mma_supports(n_heads, n_kv_heads, head_dim):
+        return attention_plain(q, n_heads, n_kv_heads, head_dim, k_pages, v_pages, page_table, seq_of_token,
+                               positions, scale, window, max_ctx_len, sinks=sinks)
+    out = torch.empty((T, n_heads * head_dim), dtype=q.dtype, device=dev)
+    if max_new_tokens == 1 and B <= 1024:
+        _need(T == B, "one token per sequence expected")
+        blocks = min(-(-max_ctx_len // PAGE), -(-window // PAGE) + 1 + -(-sinks // PAGE))
+        cluster, groups, n_ctas = _bounded_decode_plan(B, n_kv_heads, n_heads, head_dim, blocks, splits, cluster, groups, sms())
+        part_o, part_ml, tickets = _decode_scratch(B, n_kv_heads, n_heads, head_dim, n_ctas, cluster, groups, dev)
+        _check("attention_decode_bounded", lib.wpc_attention_decode_bounded(
+            _p(q), q.stride(0), _p(out), out.stride(0), _p(k_pages), _p(v_pages), _p(page_table), page_table.shape[1],
+            _p(ctx_lens), B, n_heads, n_kv_heads, head_dim, ctypes.c_float(scale), window, sinks, n_ctas, cluster, groups,
+            _p(part_o), _p(part_ml), _p(tickets), B * n_kv_heads, _p(None), 0, _p(None), _stream()))
+    elif (not mma_only and lib.wpc_attention_prefill_tc_supports(n_heads, n_kv_heads, head_dim)
+          and q.stride(0) % 8 == 0 and q.data_ptr() % 16 == 0):
+        _, _, status = workspace(dev)
+        _check("attention_prefill_tc_bounded", lib.wpc_attention_prefill_tc_bounded(
+            _p(q), q.stride(0), _p(out), out.stride(0), _p(k_pages), _p(v_pages), _p(page_table), page_table.shape[1],
+            _p(cu_seqlens), _p(ctx_lens), B, max_new_tokens, n_heads, n_kv_heads, head_dim, ctypes.c_float(scale), window,
+            sinks, _p(None), _p(status), k_pages.shape[0], _stream()))
+    else:
+        _check("attention_prefill_bounded", lib.wpc_attention_prefill_bounded(
+            _p(q), q.stride(0), _p(out), out.stride(0), _p(k_pages), _p(v_pages), _p(page_table), page_table.shape[1],
+            _p(cu_seqlens), _p(ctx_lens), B, max_new_tokens, n_heads, n_kv_heads, head_dim, ctypes.c_float(scale), window,
+            sinks, _p(None), _stream()))
+    return out
+
+
+def _attention_with_sums(q, n_heads, n_kv_heads, head_dim, k_pages, v_pages, page_table, cu_seqlens, ctx_lens,
+                         seq_of_token, positions, scale, window, max_new_tokens, max_ctx_len, splits, mma_only,
+                         cluster, groups, sinks, weight_sums, stored_positions, token_positions) -> torch.Tensor:
+    _need(weight_sums is not None and stored_positions is not None and token_positions is not None,
+          "weight_sums, stored_positions and token_positions come together")
+    _need(not window and not sinks, "weights are summed over a cache that keeps everything: no window, no sinks")
+    _check_step(q, n_heads, n_kv_heads, head_dim, k_pages, v_pages, page_table, cu_seqlens, ctx_lens, seq_of_token, positions)
+    T, B, dev, n_pages = q.shape[0], ctx_lens.numel(), q.device, k_pages.shape[0]
+    shape = (n_pages, n_kv_heads, PAGE)
+    _need(weight_sums.dtype == torch.float32 and tuple(weight_sums.shape) == shape and weight_sums.is_contiguous()
+          and weight_sums.device == dev, "weight_sums must be contiguous float32 [n_pages, n_kv_heads, PAGE]")
+    _need(stored_positions.dtype == torch.int32 and tuple(stored_positions.shape) == shape
+          and stored_positions.is_contiguous() and stored_positions.device == dev,
+          "stored_positions must be contiguous int32 [n_pages, n_kv_heads, PAGE]")
+    _need(token_positions.dtype == torch.int32 and token_positions.numel() == T and token_positions.is_contiguous()
+          and token_positions.device == dev, "token_positions must be contiguous int32 [T]")
+    out = torch.empty((T, n_heads * head_dim), dtype=q.dtype, device=dev)
+    if T == 0:
+        return out
+    lib = library()
+    _, _, status = workspace(dev)
+    fast = q.dtype == torch.bfloat16 and bool(lib.wpc_attention_mma_supports(n_heads, n_kv_heads, head_dim))
+    if fast and max_new_tokens == 1 and B <= 1024:
+        # a decode step: the scores stay in scratch memory until the rows' maxima and sums are known
+        _need(T == B, "one token per sequence expected")
+        blocks = -(-max_ctx_len // PAGE)
+        cluster, groups, n_ctas = _bounded_decode_plan(B, n_kv_heads, n_heads, head_dim, blocks, splits, cluster, groups, sms())
+        part_o, part_ml, tickets = _decode_scratch(B, n_kv_heads, n_heads, head_dim, n_ctas, cluster, groups, dev)
+        scratch = torch.empty((B * n_heads * (blocks * PAGE + 2),), dtype=torch.float32, device=dev)
+        row_ml = scratch[B * n_heads * blocks * PAGE:]
+        _check("attention_decode_bounded", lib.wpc_attention_decode_bounded(
+            _p(q), q.stride(0), _p(out), out.stride(0), _p(k_pages), _p(v_pages), _p(page_table), page_table.shape[1],
+            _p(ctx_lens), B, n_heads, n_kv_heads, head_dim, ctypes.c_float(scale), 0, 0, n_ctas, cluster, groups,
+            _p(part_o), _p(part_ml), _p(tickets), B * n_kv_heads, _p(scratch), blocks * PAGE, _p(row_ml), _stream()))
+        _check("weight_sums_decode", lib.wpc_weight_sums_decode(
+            _p(scratch), blocks * PAGE, _p(row_ml), _p(page_table), page_table.shape[1], _p(ctx_lens), _p(token_positions),
+            B, n_heads, n_kv_heads, max_ctx_len, n_pages, _p(weight_sums), _p(stored_positions), _p(status), _stream()))
+        return out
+    lse = torch.empty((T, n_heads), dtype=torch.float32, device=dev)
+    if not fast:
+        attention_plain(q, n_heads, n_kv_heads, head_dim, k_pages, v_pages, page_table, seq_of_token, positions, scale,
+                        None, max_ctx_len, lse=lse, out=out)
+    elif (not mma_only and lib.wpc_attention_prefill_tc_supports(n_heads, n_kv_heads, head_dim)
+          and q.stride(0) % 8 == 0 and q.data_ptr() % 16 == 0):
+        _check("attention_prefill_tc_bounded", lib.wpc_attention_prefill_tc_bounded(
+            _p(q), q.stride(0), _p(out), out.stride(0), _p(k_pages), _p(v_pages), _p(page_table), page_table.shape[1],
+            _p(cu_seqlens), _p(ctx_lens), B, max_new_tokens, n_heads, n_kv_heads, head_dim, ctypes.c_float(scale), 0, 0,
+            _p(lse), _p(status), n_pages, _stream()))
+    else:
+        _check("attention_prefill_bounded", lib.wpc_attention_prefill_bounded(
+            _p(q), q.stride(0), _p(out), out.stride(0), _p(k_pages), _p(v_pages), _p(page_table), page_table.shape[1],
+            _p(cu_seqlens), _p(ctx_lens), B, max_new_tokens, n_heads, n_kv_heads, head_dim, ctypes.c_float(scale), 0, 0,
+            _p(lse), _stream()))
+    _check("weight_sums_plain", lib.wpc_weight_sums_plain(
+        _p(q), q.stride(0), _code(q.dtype), _p(k_pages), _p(page_table), page_table.shape[1], _p(cu_seqlens), _p(ctx_lens),
+        _p(token_positions), _p(lse), B, n_heads, n_kv_heads, head_dim, ctypes.c_float(scale), max_ctx_len, n_pages,
+        _p(weight_sums), _p(stored_positions), _p(status), _stream()))
+    return out
+
+
+def _record(weight_sums, stored_positions, page_table):
+    """Checks the two records of one layer or of several and a page table; returns
+    (layers, pages, KV heads, sequences)."""
+    _need(weight_sums.is_cuda and weight_sums.dtype == torch.float32 and weight_sums.is_contiguous()
+          and weight_sums.dim() in (3, 4) and weight_sums.shape[-1] == PAGE,
+          "weight_sums must be contiguous float32 [layers, n_pages, n_kv_heads, PAGE] (or of one layer)")
+    dev = weight_sums.device
+    _need(dev.index == torch.cuda.current_device(),
+          f"the tensors lie on {dev}, but the current device is cuda:{torch.cuda.current_device()}")
+    _need(stored_positions.dtype == torch.int32 and stored_positions.shape == weight_sums.shape
+          and stored_positions.is_contiguous() and stored_positions.device == dev,
+          "stored_positions must be contiguous int32 of weight_sums' shape")
+    _need(page_table.dtype == torch.int32 and page_table.dim() == 2 and page_table.is_contiguous()
+          and page_table.device == dev, "page_table must be contiguous int32 [B, width]")
+    layers = 1 if weight_sums.dim() == 3 else weight_sums.shape[0]
+    return layers, weight_sums.shape[-3], weight_sums.shape[-2], page_table.shape[0]
+
+
+def select_kept(weight_sums: torch.Tensor, stored_positions: torch.Tensor, page_table: torch.Tensor,
+                stored_lens: torch.Tensor, next_positions: torch.Tensor, keep: int, sinks: int, recent: int) -> torch.Tensor:
+    """Which entries of each sequence stay when its cache is cut down to `keep` of them, for every
+    layer and KV head: the first `sinks` positions, the last `recent` positions (those from
+    next_positions[b] - recent on), and of the others the entries with the greatest
+    `weight_sums`, ties to the one stored first (a NaN counts as -inf).
+
+    weight_sums, stored_positions: [layers, n_pages, n_kv_heads, PAGE] or of one layer, as
+    `attention` keeps them; page_table int32 [B, width]; stored_lens and next_positions int32 [B]:
+    entries that a sequence holds, and the position of its next token.  Returns int32
+    [layers, B, n_kv_heads, keep] (without `layers` for one layer): at place i the stored index of
+    the entry that belongs there, i itself where it may stay, -1 behind a sequence shorter than
+    `keep`.  Entries from `keep` on that stay are spread over the holes in order (`move_kept_`)."""
+    _need(keep >= 1 and sinks >= 0 and recent >= 0 and sinks + recent <= keep,
+          f"keep must be at least 1 and hold the sinks and the recent positions, got keep {keep}, sinks {sinks}, "
+          f"recent {recent}")
+    layers, n_pages, n_kv, B = _record(weight_sums, stored_positions, page_table)
+    dev = weight_sums.device
+    for name, t in (("stored_lens", stored_lens), ("next_positions", next_positions)):
+        _need(t.dtype == torch.int32 and t.numel() == B and t.is_contiguous() and t.device == dev,
+              f"{name} must be contiguous int32 [B]")
+    kept = torch.empty((layers, B, n_kv, keep), dtype=torch.int32, device=dev)
+    if B:
+        _, _, status = workspace(dev)
+        _check("select_kept", library().wpc_select_kept(
+            _p(weight_sums), _p(stored_positions), _p(page_table), page_table.shape[1], _p(stored_lens), _p(next_positions),
+            layers, B, n_kv, n_pages, keep, sinks, recent, _p(kept), _p(status), _stream()))
+    return kept if weight_sums.dim() == 4 else kept[0]
+
+
+def move_kept_(k_pages: torch.Tensor, v_pages: torch.Tensor, weight_sums: torch.Tensor, stored_positions: torch.Tensor,
+               page_table: torch.Tensor, kept: torch.Tensor) -> None:
+    """Moves the entries that `select_kept` placed elsewhere than they are: keys, values, sums and
+    positions of entry kept[.., i] go to place i of their sequence and KV head, in place.  Every
+    kept[.., i] is i, -1 (nothing), or at least `keep`, kept's last size: an entry that is named
+    otherwise, or that has no page, stays where it is, and the device error word says 1001.
+    Afterwards the first `keep` places hold what was kept, and the pages behind them may go."""
+    layers, n_pages, n_kv, B = _record(weight_sums, stored_positions, page_table)
+    dev, lead = weight_sums.device, tuple(weight_sums.shape[:-3])
+    for name, t in (("k_pages", k_pages), ("v_pages", v_pages)):
+        _need(t.dim() == weight_sums.dim() + 1 and tuple(t.shape[:-1]) == tuple(weight_sums.shape) and t.is_contiguous()
+              and t.device == dev and t.dtype in (torch.float32, torch.bfloat16),
+              f"{name} must be contiguous [.., n_pages, n_kv_heads, PAGE, head_dim] like weight_sums")
+    _need(kept.dtype == torch.int32 and kept.is_contiguous() and kept.device == dev
+          and kept.dim() == weight_sums.dim() and tuple(kept.shape[:-1]) == lead + (B, n_kv),
+          "kept must be contiguous int32 [.., B, n_kv_heads, keep]")
+    if not kept.numel():
+        return
+    _, _, status = workspace(dev)
+    _check("move_kept", library().wpc_move_kept(
+        _p(k_pages), _p(v_pages), k_pages.shape[-1] * k_pages.element_size(), v_pages.shape[-1] * v_pages.element_size(),
+        _p(weight_sums), _p(stored_positions), _p(page_table), page_table.shape[1], _p(kept), layers, B, n_kv, n_pages,
+        kept.shape[-1], _p(status), _stream()))
 
 
 def plan_decode_ctas(n_seqs: int, n_kv_heads: int, max_ctx_len: int, window: Optional[int],
@@ -804,26 +1043,31 @@ def plan_decode_cluster(n_seqs: int, n_kv_heads: int, n_heads: int, head_dim: in
 
 
 def attention_plain(q, n_heads, n_kv_heads, head_dim, k_pages, v_pages, page_table, seq_of_token, positions,
-                    scale, window, max_ctx_len: Optional[int] = None, splits: Optional[int] = None) -> torch.Tensor:
+                    scale, window, max_ctx_len: Optional[int] = None, splits: Optional[int] = None, sinks: int = 0,
+                    lse: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """The attention of the 32-bit path and the plain twin of the fast kernels: a block to each
     (token, head).  With few tokens and long contexts (`max_ctx_len`, the longest sequence of
     the step) several blocks share a query's keys, about 256 each and no more blocks than fill
-    the device twice (`splits` forces their number); their parts are added in order."""
+    the device twice (`splits` forces their number); their parts are added in order.  `sinks`: see
+    `attention`; `lse` (float32 [T, n_heads]) gets maximum + log2(sum) of each row's scores in
+    units of log 2; `out`: where the result goes (contiguous)."""
     _rows(q, "q")
     _need(q.shape[1] >= n_heads * head_dim, "q is too narrow")
     _need(k_pages.is_contiguous() and v_pages.is_contiguous() and k_pages.dtype == q.dtype, "pages: wrong type")
     T = q.shape[0]
-    out = torch.empty((T, n_heads * head_dim), dtype=q.dtype, device=q.device)
+    if out is None:
+        out = torch.empty((T, n_heads * head_dim), dtype=q.dtype, device=q.device)
+    sinks = sinks if window else 0
     if splits is None:
-        keys = min(max_ctx_len or 0, window or (max_ctx_len or 0))
+        keys = min(max_ctx_len or 0, window + sinks if window else (max_ctx_len or 0))
         splits = max(1, min(keys // 256, 2 * sms() // max(T * n_heads, 1)))
     part = None
     if splits > 1:
         part = torch.empty((T * n_heads * splits * (head_dim + 2),), dtype=torch.float32, device=q.device)
-    _check("attention_plain", library().wpc_attention_plain(
+    _check("attention_plain", library().wpc_attention_plain_bounded(
         _p(q), q.stride(0), _p(out), out.stride(0), _code(q.dtype), _p(k_pages), _p(v_pages), _p(page_table),
         page_table.shape[1], _p(seq_of_token), _p(positions), T, n_heads, n_kv_heads, head_dim,
-        ctypes.c_float(scale), int(window or 0), int(splits), _p(part), _stream()))
+        ctypes.c_float(scale), int(window or 0), int(sinks), int(splits), _p(part), _p(lse), _stream()))
     return out
 
 
