@@ -506,3 +506,27 @@ def test_refusals():
     refused("kept must be", ops.move_kept_, k, v, sums, stored, table, kept.long())
     refused("page_table", ops.move_kept_, k, v, sums, stored, table.long(), kept)
     assert ops.device_status() == 0
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_starved_sums_return_with_1004_and_the_next_ones_are_right(hd):
+    """The prompt's kernels start no copies, so their waits run out; nothing hangs, the error word says
+    so, and the next call is right."""
+    s = Step(torch.bfloat16, 14, 2, hd, [400], [390], seed=3)
+    told, want = s.pos, s.want()
+    old, _ = s.record()
+    sums, stored = s.record()
+    s.attend(weight_sums=sums, stored_positions=stored, token_positions=told)
+    torch.cuda.synchronize()
+    try:
+        ops.set_wait_policy(3_000_000, starve=True)
+        s.attend(weight_sums=sums, stored_positions=stored, token_positions=told)
+        torch.cuda.synchronize()
+    finally:
+        ops.set_wait_policy()
+    with pytest.raises(ops.KernelError, match="1004"):
+        ops.check_device_status()
+    sums, stored = s.record()
+    s.attend(weight_sums=sums, stored_positions=stored, token_positions=told)
+    s.check_sums(sums, stored, old, want, told)
+    assert ops.device_status() == 0

@@ -1329,6 +1329,20 @@ int tensor_map(const void* ptr, int rows, int cols, int ld, int box_rows, CUtens
   return 0;
 }
 
+int tensor_map_heads(const void* ptr, int tokens, int heads, int hd, int ld, int box_tokens, int box_heads,
+                     CUtensorMap* out) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return WPC_ERR_UNSUPPORTED;
+  cuuint64_t dims[3] = {(cuuint64_t)hd, (cuuint64_t)heads, (cuuint64_t)tokens};
+  cuuint64_t strides[2] = {(cuuint64_t)hd * 2, (cuuint64_t)ld * 2};
+  cuuint32_t box[3] = {(cuuint32_t)BK, (cuuint32_t)box_heads, (cuuint32_t)box_tokens};
+  cuuint32_t estr[3] = {1, 1, 1};
+  const CUresult r = fn(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(ptr), dims, strides, box, estr,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? 0 : WPC_ERR_UNSUPPORTED;
+}
+
 // Upper limit of the ring depth (a tuning knob; MAX_STAGES by default).
 static int g_stage_limit = MAX_STAGES;
 

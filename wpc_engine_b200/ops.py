@@ -843,6 +843,11 @@ def _attention_with_sums(q, n_heads, n_kv_heads, head_dim, k_pages, v_pages, pag
             _p(q), q.stride(0), _p(out), out.stride(0), _p(k_pages), _p(v_pages), _p(page_table), page_table.shape[1],
             _p(cu_seqlens), _p(ctx_lens), B, max_new_tokens, n_heads, n_kv_heads, head_dim, ctypes.c_float(scale), 0, 0,
             _p(lse), _p(status), n_pages, _stream()))
+        _check("weight_sums_tc", lib.wpc_weight_sums_tc(
+            _p(q), q.stride(0), T, _p(k_pages), _p(page_table), page_table.shape[1], _p(cu_seqlens), _p(ctx_lens),
+            _p(token_positions), _p(lse), B, n_heads, n_kv_heads, head_dim, ctypes.c_float(scale), max_new_tokens,
+            max_ctx_len, n_pages, _p(weight_sums), _p(stored_positions), _p(status), _stream()))
+        return out
     else:
         _check("attention_prefill_bounded", lib.wpc_attention_prefill_bounded(
             _p(q), q.stride(0), _p(out), out.stride(0), _p(k_pages), _p(v_pages), _p(page_table), page_table.shape[1],
