@@ -273,7 +273,8 @@ def eviction_case(layers, nkv, lens, seed, hd=8, dtype=torch.bfloat16, special=T
 
 @pytest.mark.parametrize("lens,keep,sinks,recent", [
     ([200, 64, 65, 0, 1, 130], 64, 4, 10), ([200, 300], 100, 0, 0), ([129, 500], 1, 0, 1), ([90], 89, 30, 59),
-    ([1000, 40], 513, 16, 100), ([700], 700, 1, 1), ([300], 800, 5, 5), ([2000, 1900], 1025, 4, 900)])
+    ([1000, 40], 513, 16, 100), ([700], 700, 1, 1), ([300], 800, 5, 5), ([2000, 1900], 1025, 4, 900),
+    ([4096, 4033], 4000, 4, 20), ([8129, 300], 77, 4, 20), ([9000, 20], 4097, 1, 4000)])
 @pytest.mark.parametrize("layers", [1, 3])
 def test_select_and_move(lens, keep, sinks, recent, layers):
     sums, stored, table, k, v = eviction_case(layers, 2, lens, keep + layers)
@@ -300,6 +301,45 @@ def test_select_and_move_of_one_layer_take_tensors_without_that_dimension():
                for a, b in zip(one, (k, v, sums, stored)))
 
 
+def test_select_with_more_to_keep_than_the_table_holds():
+    sums, stored, table, _, _ = eviction_case(2, 2, [200, 64], 1)
+    kept = ops.select_kept(sums, stored, table, ints([200, 64]), ints([200, 200]), 60000, 1, 1)
+    i = torch.arange(60000)
+    for b, n in enumerate((200, 64)):
+        assert torch.equal(kept[:, b].cpu().long(), torch.where(i < n, i, -1).expand(2, 2, 60000))
+
+
+def test_records_that_begin_at_odd_addresses():
+    lens = [300, 200]
+    sums, stored, table, k, v = eviction_case(2, 2, lens, 1)
+    odd = [torch.empty(t.numel() + 1, dtype=t.dtype, device=DEV)[1:].view(t.shape).copy_(t) for t in (sums, stored, k, v)]
+    want = ops.select_kept(sums, stored, table, ints(lens), ints([1500, 1500]), 100, 2, 30)
+    kept = ops.select_kept(odd[0], odd[1], table, ints(lens), ints([1500, 1500]), 100, 2, 30)
+    assert torch.equal(kept, want)
+    ops.move_kept_(k, v, sums, stored, table, want)
+    ops.move_kept_(odd[2], odd[3], odd[0], odd[1], table, kept)
+    for a, b in zip(odd, (sums, stored, k, v)):
+        assert torch.equal(torch.nan_to_num(a.float()), torch.nan_to_num(b.float()))
+
+
+def test_queries_that_begin_at_odd_addresses():
+    for new in ([1, 1], [60, 130]):
+        for sums in (False, True):
+            s = Step(torch.bfloat16, 14, 2, 64, [300, 170], new, None if sums else 100, 0 if sums else 5, seed=1)
+            record = s.record()
+            kw = dict(weight_sums=record[0], stored_positions=record[1], token_positions=s.pos) if sums else dict(sinks=5)
+            want = s.want()
+            for offset, pad in ((1, 1), (2, 2), (4, 4), (0, 1), (0, 2)):
+                T, width = s.q.shape
+                wide = torch.zeros(T * (width + pad) + offset, dtype=s.q.dtype, device=DEV)
+                q = wide[offset:].view(T, width + pad)[:, :width]
+                q.copy_(s.q)
+                whole, s.q = s.q, q
+                s.check_out(s.attend(**kw), want)
+                s.q = whole
+    assert ops.device_status() == 0
+
+
 def test_select_with_all_protected_or_all_equal_or_none_finite():
     lens, keep = [400], 100
     for fill, recent in ((1.0, 0), (math.nan, 0), (-math.inf, 3), (2.0, 100)):
@@ -311,11 +351,15 @@ def test_select_with_all_protected_or_all_equal_or_none_finite():
         assert torch.equal(kept.cpu().long(), plain.select(sums, stored, table, lens, [1500], keep, 0, recent))
 
 
-def test_select_of_more_entries_than_shared_memory_holds():
-    lens = [52000, 51000]
+@pytest.mark.parametrize("lens,keep", [([32704, 31000], 900), ([32700], 24576), ([32700], 24577), ([52000, 51000], 900),
+                                       ([52000], 51200)])
+def test_select_of_many_entries(lens, keep):
+    """Keys in registers up to 32,768 entries (and the places of what is kept in shared memory), read
+    again for every digit beyond."""
     sums, stored, table, _, _ = eviction_case(1, 1, lens, 8, hd=1)
-    kept = ops.select_kept(sums, stored, table, ints(lens), ints([2500, 2500]), 900, 4, 10)
-    assert torch.equal(kept.cpu().long(), plain.select(sums, stored, table, lens, [2500, 2500], 900, 4, 10))
+    after = [2500] * len(lens)
+    kept = ops.select_kept(sums, stored, table, ints(lens), ints(after), keep, 4, 10)
+    assert torch.equal(kept.cpu().long(), plain.select(sums, stored, table, lens, after, keep, 4, 10))
 
 
 @pytest.mark.parametrize("dtype,hd", [(torch.bfloat16, 128), (torch.bfloat16, 3), (torch.float32, 5), (torch.float32, 64),
@@ -498,7 +542,6 @@ def test_refusals():
     refused("stored_lens", ops.select_kept, sums, stored, table, lens.long(), after, 10, 1, 1)
     refused("next_positions", ops.select_kept, sums, stored, table, lens, ints([1, 2]), 10, 1, 1)
     refused("stored_positions", ops.select_kept, sums, stored[0], table, lens, after, 10, 1, 1)
-    refused("beyond", ops.select_kept, sums, stored, table, lens, after, 60000, 1, 1)
     kept = ops.select_kept(sums, stored, table, lens, after, 64, 1, 1)
     refused("k_pages", ops.move_kept_, k[0], v, sums, stored, table, kept)
     refused("v_pages", ops.move_kept_, k, v.half(), sums, stored, table, kept)

@@ -105,12 +105,15 @@ int wpc_attention_prefill_tc_bounded(const void* q, int q_stride, void* out, int
 // decode: cluster 0: n_ctas CTAs share all pages (part_o, part_ml, counters as in
 // wpc_attention_decode); else `groups` clusters of that size to a pair (as in
 // wpc_attention_decode_cluster).  scores: float32 [B * nkv][nh / nkv][score_stride], score_stride a
-// multiple of 64 that covers the longest context; row_ml: float32 [B][nh][2].
+// multiple of 64 that covers the longest context max_ctx; row_ml: float32 [B][nh][2].  With scores a
+// second kernel (wpc_weight_sums_decode, which says what the last arguments are) follows.
 int wpc_attention_decode_bounded(const void* q, int q_stride, void* out, int out_stride, const void* k_pages,
                                  const void* v_pages, const int* page_table, int table_width, const int* ctx_lens,
                                  int B, int nh, int nkv, int hd, float scale, int window, int sinks, int n_ctas,
                                  int cluster, int groups, float* part_o, float* part_ml, int* counters, int n_counters,
-                                 float* scores, int score_stride, float* row_ml, cudaStream_t stream);
+                                 float* scores, int score_stride, float* row_ml, const int* token_positions, int max_ctx,
+                                 int n_pages, float* weight_sums, int* stored_positions, int* status,
+                                 cudaStream_t stream);
 int wpc_attention_prefill_bounded(const void* q, int q_stride, void* out, int out_stride, const void* k_pages,
                                   const void* v_pages, const int* page_table, int table_width, const int* cu_seqlens,
                                   const int* ctx_lens, int B, int max_new, int nh, int nkv, int hd, float scale,

@@ -11,13 +11,11 @@
 
 using namespace wpc;
 
-extern "C" {
-
-int wpc_attention_decode_bounded(const void* q, int q_stride, void* out, int out_stride, const void* k_pages,
-                                 const void* v_pages, const int* page_table, int table_width, const int* ctx_lens,
-                                 int B, int nh, int nkv, int hd, float scale, int window, int sinks, int n_ctas,
-                                 int cluster, int groups, float* part_o, float* part_ml, int* counters, int n_counters,
-                                 float* scores, int score_stride, float* row_ml, cudaStream_t stream) {
+static int decode_bounded(const void* q, int q_stride, void* out, int out_stride, const void* k_pages,
+                          const void* v_pages, const int* page_table, int table_width, const int* ctx_lens,
+                          int B, int nh, int nkv, int hd, float scale, int window, int sinks, int n_ctas,
+                          int cluster, int groups, float* part_o, float* part_ml, int* counters, int n_counters,
+                          float* scores, int score_stride, float* row_ml, cudaStream_t stream) {
   if (B <= 0) return 0;
   if (!wpc_attention_mma_supports(nh, nkv, hd) || (q_stride % 2) || (out_stride % 2)) return WPC_ERR_UNSUPPORTED;
   const bool sums = scores != nullptr;
@@ -50,6 +48,23 @@ int wpc_attention_decode_bounded(const void* q, int q_stride, void* out, int out
   WPC_DISPATCH_HD(hd, fa::launch_decode<HD, fa::MODE_SINKS>(
       q, q_stride, out, out_stride, k_pages, v_pages, page_table, table_width, ctx_lens, B, nh, nkv, scale, window,
       n_ctas, part_o, part_ml, counters, x, stream));
+}
+
+extern "C" {
+
+int wpc_attention_decode_bounded(const void* q, int q_stride, void* out, int out_stride, const void* k_pages,
+                                 const void* v_pages, const int* page_table, int table_width, const int* ctx_lens,
+                                 int B, int nh, int nkv, int hd, float scale, int window, int sinks, int n_ctas,
+                                 int cluster, int groups, float* part_o, float* part_ml, int* counters, int n_counters,
+                                 float* scores, int score_stride, float* row_ml, const int* token_positions, int max_ctx,
+                                 int n_pages, float* weight_sums, int* stored_positions, int* status,
+                                 cudaStream_t stream) {
+  const int rc = decode_bounded(q, q_stride, out, out_stride, k_pages, v_pages, page_table, table_width, ctx_lens, B, nh,
+                                nkv, hd, scale, window, sinks, n_ctas, cluster, groups, part_o, part_ml, counters,
+                                n_counters, scores, score_stride, row_ml, stream);
+  if (rc || !scores) return rc;
+  return wpc_weight_sums_decode(scores, score_stride, row_ml, page_table, table_width, ctx_lens, token_positions, B, nh,
+                                nkv, max_ctx, n_pages, weight_sums, stored_positions, status, stream);
 }
 
 int wpc_attention_prefill_bounded(const void* q, int q_stride, void* out, int out_stride, const void* k_pages,

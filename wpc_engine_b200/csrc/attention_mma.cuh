@@ -395,7 +395,7 @@ decode_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, __nv_bfloat16* 
       }
       cp_async_commit();
     }
-    const __nv_bfloat16* qtok = q + (size_t)b * q_stride + (size_t)g * n_rep * HD;
+    const __nv_bfloat16* qtok = after_wait(q) + (size_t)b * q_stride + (size_t)g * n_rep * HD;
     uint32_t qf[HD / 16][4];
     load_q<HD>(qf, r_lo < n_rep ? qtok + r_lo * HD : nullptr, r_hi < n_rep ? qtok + r_hi * HD : nullptr, lane);
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
@@ -653,7 +653,7 @@ decode_cluster_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, __nv_bf
     cp_async_commit();
   }
   const int r_lo = lane >> 2, r_hi = r_lo + 8;                        // rows = heads of the group
-  const __nv_bfloat16* qtok = q + (size_t)b * q_stride + (size_t)g * n_rep * HD;
+  const __nv_bfloat16* qtok = after_wait(q) + (size_t)b * q_stride + (size_t)g * n_rep * HD;
   uint32_t qf[HD / 16][4];
   load_q<HD>(qf, r_lo < n_rep ? qtok + r_lo * HD : nullptr, r_hi < n_rep ? qtok + r_hi * HD : nullptr, lane);
   float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
@@ -858,6 +858,7 @@ prefill_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, __nv_bfloat16*
   const int h_lo = g * n_rep + (v_lo ? r_lo % n_rep : 0), h_hi = g * n_rep + (v_hi ? r_hi % n_rep : 0);
   const int p_lo = start + t_lo, p_hi = start + t_hi;                // positions of the two rows
   uint32_t qf[HD / 16][4];
+  q = after_wait(q);
   load_q<HD>(qf, v_lo ? q + (size_t)(tok0 + t_lo) * q_stride + (size_t)h_lo * HD : nullptr,
              v_hi ? q + (size_t)(tok0 + t_hi) * q_stride + (size_t)h_hi * HD : nullptr, lane);
 

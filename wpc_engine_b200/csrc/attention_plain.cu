@@ -34,6 +34,9 @@ attention_plain_kernel(const T* __restrict__ q, int q_stride, T* __restrict__ ou
                        float* __restrict__ part) {
   pdl_trigger();
   pdl_wait();
+  q = after_wait(q);
+  k_pages = after_wait(k_pages);
+  v_pages = after_wait(v_pages);
   extern __shared__ float smem[];
   float* qs = smem;                    // [hd]
   float* ps = smem + hd;               // [AP_CHUNK]
@@ -143,7 +146,7 @@ __global__ void attention_plain_combine_kernel(const float* __restrict__ part, T
   pdl_trigger();
   pdl_wait();
   const int t = blockIdx.x, h = blockIdx.y;
-  const float* prow = part + ((size_t)t * nh + h) * n_splits * (hd + 2);
+  const float* prow = after_wait(part) + ((size_t)t * nh + h) * n_splits * (hd + 2);
   float m = -INFINITY;
   for (int z = 0; z < n_splits; ++z) m = fmaxf(m, prow[(size_t)z * (hd + 2) + hd]);
   if (lse && threadIdx.x == 0) {

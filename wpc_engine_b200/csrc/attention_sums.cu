@@ -25,7 +25,7 @@ constexpr float SUMS_LOG2E = 1.4426950408889634f;
 constexpr int SUMS_THREADS = 256;
 
 __global__ void __launch_bounds__(SUMS_THREADS)
-decode_sums_kernel(const float* __restrict__ scores, int score_stride, const float2* __restrict__ row_ml,
+decode_sums_kernel(const float* scores, int score_stride, const float2* row_ml,
                    const int* __restrict__ ctx_lens, int nh, int nkv, SumsTarget t) {
   pdl_trigger();
   pdl_wait();
@@ -48,8 +48,8 @@ constexpr int SUMS_ROWS = 16;       // (token, head) rows of q in shared memory 
 
 template <typename T>
 __global__ void __launch_bounds__(SUMS_THREADS)
-sums_plain_kernel(const T* __restrict__ q, int q_stride, const T* __restrict__ k_pages,
-                  const int* __restrict__ cu_seqlens, const int* __restrict__ ctx_lens, const float* __restrict__ lse,
+sums_plain_kernel(const T* q, int q_stride, const T* k_pages,
+                  const int* __restrict__ cu_seqlens, const int* __restrict__ ctx_lens, const float* lse,
                   int nh, int nkv, int hd, float scale, SumsTarget t) {
   pdl_trigger();
   pdl_wait();

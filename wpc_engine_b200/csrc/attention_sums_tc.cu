@@ -68,7 +68,7 @@ __device__ __forceinline__ bool all_of_128(bool ok) {
 template <int HD>
 __global__ void __launch_bounds__(ST_THREADS, 2)
 prefill_sums_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_q,
-                    const int* __restrict__ cu_seqlens, const int* __restrict__ ctx_lens, const float* __restrict__ lse,
+                    const int* __restrict__ cu_seqlens, const int* __restrict__ ctx_lens, const float* lse,
                     int nh, int nkv, int C, int tile_tokens, float scale_log2, const SumsTarget t,
                     unsigned long long wait_ns, int starve, int late_trigger) {
   using W = StCfg<HD>;

@@ -261,7 +261,7 @@ prefill_ws_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     const int lo_row = (window > 0 && p_row - window + 1 > 0) ? p_row - window + 1 : 0;
     const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
     {
-      const __nv_bfloat16* src = q + (size_t)(tok0 + t_row) * q_stride + (size_t)h_row * HD;
+      const __nv_bfloat16* src = after_wait(q) + (size_t)(tok0 + t_row) * q_stride + (size_t)h_row * HD;
       uint8_t* my_q = base + t * C::Q_BYTES;
 #pragma unroll
       for (int c = 0; c < HD / 8; ++c) {

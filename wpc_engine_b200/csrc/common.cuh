@@ -138,7 +138,15 @@ __device__ __forceinline__ void cluster_wait() {
 // weights while the kernel before it is still finishing; pdl_wait() returns once that kernel
 // has completed and its writes are visible.  Without the attribute both calls do nothing.
 __device__ __forceinline__ void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+// (What an earlier kernel wrote must not be read through a `const T* __restrict__` parameter as it is:
+// such loads count as loads of constants, and the compiler may move them ahead of pdl_wait().
+// after_wait(p), called behind it, gives a pointer whose loads stay behind it.)
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+template <typename T>
+__device__ __forceinline__ T* after_wait(T* p) {
+  asm volatile("" : "+l"(p)::"memory");
+  return p;
+}
 
 inline int& pdl_enabled() {
   static int on = 1;

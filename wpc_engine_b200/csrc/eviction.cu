@@ -17,7 +17,6 @@
 
 namespace wpc {
 
-constexpr int SEL_THREADS = 512;
 constexpr uint32_t SEL_PROTECTED = 0xffffffffu;
 
 __device__ __forceinline__ uint32_t order_key(float w) {
@@ -26,7 +25,25 @@ __device__ __forceinline__ uint32_t order_key(float w) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;        // at most 0xff800000, for +inf
 }
 
-// Exclusive sum over the block's threads of `v`; *total: the sum of all.  red: 17 ints.
+// Where the entries of a (layer, sequence, KV head) are, and their keys.
+struct Entries {
+  const float* sums;               // of the layer
+  const int* positions;
+  const int* table;                // of the sequence
+  int nkv, g, n_pages, sinks, first_recent;
+  __device__ __forceinline__ uint32_t key_of(float w, int p) const {
+    return p < sinks || p >= first_recent ? SEL_PROTECTED : order_key(w);
+  }
+  // place of entry i in the records, -1 without a page
+  __device__ __forceinline__ long at(int i) const {
+    const int page = table[i / WPC_PAGE];
+    return page < 0 || page >= n_pages ? -1 : ((long)page * nkv + g) * WPC_PAGE + i % WPC_PAGE;
+  }
+};
+
+// Exclusive sum of `v` over the block's NT threads; *total: the sum of all.  red: 32 ints of this
+// call's own (two arrays in turn do for any number of calls: each has a barrier inside).
+template <int NT>
 __device__ __forceinline__ int block_scan(int v, int* red, int* total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int incl = v;
@@ -35,66 +52,184 @@ __device__ __forceinline__ int block_scan(int v, int* red, int* total) {
     const int t = __shfl_up_sync(0xffffffffu, incl, o);
     if (lane >= o) incl += t;
   }
-  __syncthreads();
   if (lane == 31) red[warp] = incl;
   __syncthreads();
-  int before = 0, all = 0;
+  int w = lane < NT / 32 ? red[lane] : 0;
 #pragma unroll
-  for (int i = 0; i < SEL_THREADS / 32; ++i) {
-    const int x = red[i];
-    before += i < warp ? x : 0;
-    all += x;
+  for (int o = 1; o < 32; o <<= 1) {
+    const int t = __shfl_up_sync(0xffffffffu, w, o);
+    if (lane >= o) w += t;
   }
-  *total = all;
-  return before + incl - v;
+  *total = __shfl_sync(0xffffffffu, w, 31);
+  const int before = __shfl_sync(0xffffffffu, w, (warp + 31) & 31);
+  return (warp ? before : 0) + incl - v;
 }
 
-// A block to a (layer, sequence, KV head).  Shared memory: the holes' places (keep ints), and
-// with KEYS the keys of all entries (else they are made again from memory each time).
-template <bool KEYS>
-__global__ void __launch_bounds__(SEL_THREADS)
-select_kept_kernel(const float* __restrict__ weight_sums, const int* __restrict__ stored_positions, size_t layer_stride,
+// ---- up to NT * ITEMS entries: their keys stay in registers ------------------------------------------
+// A block to a (layer, sequence, KV head); a thread owns ITEMS consecutive entries, which lie in one
+// page.  The keep-th greatest key is found in three digits of 11, 11 and 10 bits by histograms in
+// shared memory (with 8-bit digits the first one holds hardly more than the exponent, and
+// nearly all additions of a block would meet in a few bins); a digit whose bin is wanted whole
+// ends the search.  Then two scans give ties, holes and movers their ranks.
+template <int NT, int ITEMS>
+__global__ void __launch_bounds__(NT)
+select_kept_kernel(const float* weight_sums, const int* stored_positions, size_t layer_stride,
                    const int* __restrict__ page_table, int table_width, const int* __restrict__ lens,
                    const int* __restrict__ next_positions, int nkv, int n_pages, int keep, int sinks, int recent,
-                   int* __restrict__ kept, int* __restrict__ status) {
+                   int* kept, int* status) {
+  constexpr int BINS = 2048, PER = BINS / NT;
+  pdl_trigger();
+  extern __shared__ int smem[];
+  int* const places = smem;                             // [keep] what belongs at each place
+  int* const holes = smem + keep;                       // [keep]
+  __shared__ __align__(16) int hist[BINS];
+  __shared__ int red[2][32];
+  __shared__ int s_digit, s_want, s_count;
+  const int g = blockIdx.x, b = blockIdx.y, layer = blockIdx.z, B = gridDim.y, tid = threadIdx.x;
+  for (int i = tid; i < BINS; i += NT) hist[i] = 0;
+  pdl_wait();
+  int* const out = kept + (((size_t)layer * B + b) * nkv + g) * keep;
+  const int n = min(max(lens[b], 0), table_width * WPC_PAGE);
+  if (n <= keep) {                                      // nothing has to go
+    for (int i = tid; i < keep; i += NT) out[i] = i < n ? i : -1;
+    return;
+  }
+  const Entries e{weight_sums + layer * layer_stride, stored_positions + layer * layer_stride,
+                  page_table + (size_t)b * table_width, nkv, g, n_pages, sinks, next_positions[b] - recent};
+  const int i0 = tid * ITEMS;
+  uint32_t key[ITEMS];
+#pragma unroll
+  for (int j = 0; j < ITEMS; ++j) key[j] = 0;
+  if (i0 < n) {
+    const long at = e.at(i0);
+    if (at < 0) {
+      if (status) atomicExch(status, WPC_ERR_BAD_ARGUMENT);
+    } else {
+#pragma unroll
+      for (int j = 0; j < ITEMS; j += 4) {
+        const float4 w = *(const float4*)(e.sums + at + j);
+        const int4 p = *(const int4*)(e.positions + at + j);
+        key[j] = e.key_of(w.x, p.x);
+        key[j + 1] = e.key_of(w.y, p.y);
+        key[j + 2] = e.key_of(w.z, p.z);
+        key[j + 3] = e.key_of(w.w, p.w);
+      }
+    }
+  }
+  const int mine = min(max(n - i0, 0), ITEMS);          // entries that exist
+  uint32_t prefix = 0, mask = 0;
+  int want = keep, which = 0;
+  __syncthreads();                                      // hist is zero
+#pragma unroll
+  for (int digit = 0; digit < 3; ++digit) {
+    const int shift = digit == 0 ? 21 : digit == 1 ? 10 : 0;
+    const uint32_t bins = digit == 2 ? 1023u : 2047u;
+#pragma unroll
+    for (int j = 0; j < ITEMS; ++j)
+      if (j < mine && (key[j] & mask) == prefix) atomicAdd(&hist[(key[j] >> shift) & bins], 1);
+    __syncthreads();
+    int c[PER], sum = 0;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {                     // the highest bins belong to the first thread
+      c[j] = hist[BINS - 1 - tid * PER - j];
+      hist[BINS - 1 - tid * PER - j] = 0;               // for the next digit
+      sum += c[j];
+    }
+    int total;
+    int above = block_scan<NT>(sum, red[which], &total);
+    which ^= 1;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      if (above < want && above + c[j] >= want) {
+        s_digit = BINS - 1 - tid * PER - j;
+        s_want = want - above;
+        s_count = c[j];
+      }
+      above += c[j];
+    }
+    __syncthreads();
+    prefix |= (uint32_t)s_digit << shift;
+    mask |= bins << shift;
+    want = s_want;
+    if (s_count == want) break;                         // the bin is wanted whole
+    __syncthreads();                                    // (s_digit and its like are written again)
+  }
+  const bool some_ties = s_count != want;
+
+  // ---- an entry stays if its digits are greater, or equal and it is among the first `want` of those ----
+  int total, rank = 0;
+  if (some_ties) {
+    int ties = 0;
+#pragma unroll
+    for (int j = 0; j < ITEMS; ++j) ties += j < mine && (key[j] & mask) == prefix;
+    rank = block_scan<NT>(ties, red[which], &total);
+    which ^= 1;
+  }
+  uint32_t stays = 0;
+  int n_holes = 0, n_movers = 0;
+#pragma unroll
+  for (int j = 0; j < ITEMS; ++j) {
+    const uint32_t k = key[j] & mask;
+    const bool tie = j < mine && k == prefix;
+    const bool stay = (j < mine && k > prefix) || (tie && (!some_ties || rank < want));
+    rank += tie;
+    stays |= (stay ? 1u : 0u) << j;
+    n_holes += !stay && i0 + j < keep;                  // (n > keep: every place below keep has an entry)
+    n_movers += stay && i0 + j >= keep;
+  }
+  const int ranks = block_scan<NT>(n_holes | n_movers << 16, red[which], &total);   // both at most 32,767
+  int hole = ranks & 0xffff, mover = ranks >> 16;
+#pragma unroll
+  for (int j = 0; j < ITEMS; ++j)
+    if (i0 + j < keep) {
+      if (stays >> j & 1) places[i0 + j] = i0 + j;
+      else holes[hole++] = i0 + j;
+    }
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < ITEMS; ++j)
+    if (i0 + j >= keep && (stays >> j & 1)) places[holes[mover++]] = i0 + j;
+  __syncthreads();
+  for (int i = tid; i < keep; i += NT) out[i] = places[i];
+}
+
+// ---- any number of entries ----------------------------------------------------------------------------
+// The same with the keys made anew from the records each time, eight bits a digit.
+constexpr int SEL_THREADS = 1024;
+
+__global__ void __launch_bounds__(SEL_THREADS)
+select_kept_long_kernel(const float* weight_sums, const int* stored_positions, size_t layer_stride,
+                        const int* __restrict__ page_table, int table_width, const int* __restrict__ lens,
+                        const int* __restrict__ next_positions, int nkv, int n_pages, int keep, int sinks, int recent,
+                        int* kept, int* status) {
   pdl_trigger();
   pdl_wait();
-  extern __shared__ uint32_t smem[];
-  int* holes = (int*)smem;                              // [keep]
-  uint32_t* keys = smem + keep;                         // [n]
+  extern __shared__ int smem[];
+  int* const holes = smem;                              // [keep]
   __shared__ int hist[256];
-  __shared__ int red[SEL_THREADS / 32];
+  __shared__ int red[2][32];
   __shared__ uint32_t s_digit;
   __shared__ int s_want;
   const int g = blockIdx.x, b = blockIdx.y, layer = blockIdx.z, B = gridDim.y, tid = threadIdx.x;
-  int* out = kept + (((size_t)layer * B + b) * nkv + g) * keep;
-  const int* table = page_table + (size_t)b * table_width;
+  int* const out = kept + (((size_t)layer * B + b) * nkv + g) * keep;
   const int n = min(max(lens[b], 0), table_width * WPC_PAGE);
-  if (n <= keep) {                                      // nothing has to go
+  if (n <= keep) {
     for (int i = tid; i < keep; i += SEL_THREADS) out[i] = i < n ? i : -1;
     return;
   }
-  const int first_recent = next_positions[b] - recent;
+  const Entries e{weight_sums + layer * layer_stride, stored_positions + layer * layer_stride,
+                  page_table + (size_t)b * table_width, nkv, g, n_pages, sinks, next_positions[b] - recent};
   bool bad = false;
-  auto key_of = [&](int i) -> uint32_t {
-    const int page = table[i / WPC_PAGE];
-    if (page < 0 || page >= n_pages) { bad = true; return 0u; }
-    const size_t at = layer * layer_stride + ((size_t)page * nkv + g) * WPC_PAGE + i % WPC_PAGE;
-    const int p = stored_positions[at];
-    return (p < sinks || p >= first_recent) ? SEL_PROTECTED : order_key(weight_sums[at]);
+  auto key = [&](int i) -> uint32_t {
+    const long at = e.at(i);
+    bad = bad || at < 0;
+    return at < 0 ? 0u : e.key_of(e.sums[at], e.positions[at]);
   };
-  if (KEYS) {
-    for (int i = tid; i < n; i += SEL_THREADS) keys[i] = key_of(i);
-  }
-  auto key = [&](int i) { return KEYS ? keys[i] : key_of(i); };
-
-  // ---- the keep-th greatest key, eight bits at a time; `want`: how many of those that share
-  // the digits found so far are still to be taken ----
   uint32_t prefix = 0;
   int want = keep;
   for (int shift = 24; shift >= 0; shift -= 8) {
     __syncthreads();
-    for (int i = tid; i < 256; i += SEL_THREADS) hist[i] = 0;
+    if (tid < 256) hist[tid] = 0;
     __syncthreads();
     const uint32_t mask = shift == 24 ? 0u : 0xffffffffu << (shift + 8);
     for (int i = tid; i < n; i += SEL_THREADS) {
@@ -127,19 +262,19 @@ select_kept_kernel(const float* __restrict__ weight_sums, const int* __restrict_
     prefix |= s_digit << shift;
     want = s_want;
   }
-
-  // ---- every entry: kept if its key is greater, or equal and among the first `want` of those ----
-  int ties = 0, n_holes = 0, n_movers = 0;              // of all entries before this round's
+  int ties = 0, n_holes = 0, n_movers = 0, which = 0;   // of all entries before this round's
   for (int i0 = 0; i0 < n; i0 += SEL_THREADS) {
     const int i = i0 + tid;
     const uint32_t k = i < n ? key(i) : 0u;
     const bool tie = i < n && k == prefix;
     int total;
-    const int rank = ties + block_scan(tie ? 1 : 0, red, &total);
+    const int rank = ties + block_scan<SEL_THREADS>(tie ? 1 : 0, red[which], &total);
+    which ^= 1;
     ties += total;
     const bool stays = i < n && (k > prefix || (tie && rank < want));
     const bool hole = i < keep && !stays, mover = i >= keep && stays;
-    const int at = block_scan((hole ? 1 : 0) | (mover ? 1 << 16 : 0), red, &total);
+    const int at = block_scan<SEL_THREADS>((hole ? 1 : 0) | (mover ? 1 << 16 : 0), red[which], &total);
+    which ^= 1;
     if (i < keep && stays) out[i] = i;
     if (hole) holes[n_holes + (at & 0xffff)] = i;
     n_holes += total & 0xffff;
@@ -152,25 +287,29 @@ select_kept_kernel(const float* __restrict__ weight_sums, const int* __restrict_
   if (bad && status) atomicExch(status, WPC_ERR_BAD_ARGUMENT);
 }
 
-constexpr int MOVE_THREADS = 256;
+// ---- the moves --------------------------------------------------------------------------------------------
+// A block to MOVE_PLACES places of the kept part of a (layer, sequence, KV head): it lists the moves among
+// them in shared memory, then its threads copy the listed rows, chunk by chunk, several loads
+// each before the first store (a row at a time would be a trip to memory for every row).
+constexpr int MOVE_THREADS = 256, MOVE_PLACES = 256, MOVE_DEPTH = 4;
 
-// A warp to 32 places of the kept part of a (layer, sequence, KV head).
 template <typename V>
 __global__ void __launch_bounds__(MOVE_THREADS)
-move_kept_kernel(uint8_t* __restrict__ k_pages, uint8_t* __restrict__ v_pages, int k_bytes, int v_bytes,
-                 float* __restrict__ weight_sums, int* __restrict__ stored_positions, const int* __restrict__ page_table,
-                 int table_width, const int* __restrict__ kept, int B, int nkv, int n_pages, int keep,
-                 int* __restrict__ status) {
+move_kept_kernel(V* k_pages, V* v_pages, int k_chunks, int v_chunks, float* weight_sums, int* stored_positions,
+                 const int* __restrict__ page_table, int table_width, const int* kept, int B, int nkv, int n_pages,
+                 int keep, int* status) {
   // (no early start of the kernel behind: decode attention reads pages of earlier positions ahead of its
   // dependency wait, which is right only if nothing on the stream still writes them)
+  __shared__ long s_from[MOVE_PLACES], s_to[MOVE_PLACES];
+  __shared__ int s_n;
+  if (threadIdx.x == 0) s_n = 0;
   pdl_wait();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int row = blockIdx.y;                           // (layer, sequence, KV head)
+  const int row = blockIdx.y, tid = threadIdx.x, lane = tid & 31;           // row: (layer, sequence, KV head)
   const int g = row % nkv, b = (row / nkv) % B, layer = row / (nkv * B);
-  const int i = (blockIdx.x * (MOVE_THREADS / 32) + warp) * 32 + lane;
+  const int i = blockIdx.x * MOVE_PLACES + tid;
   const int* table = page_table + (size_t)b * table_width;
   const int src = i < keep ? kept[(size_t)row * keep + i] : -1;
-  size_t from = 0, to = 0;
+  long from = 0, to = 0;
   bool moves = src >= 0 && src != i;
   if (moves) {
     const int sb = src / WPC_PAGE, db = i / WPC_PAGE;
@@ -179,19 +318,42 @@ move_kept_kernel(uint8_t* __restrict__ k_pages, uint8_t* __restrict__ v_pages, i
       moves = false;
       if (status) atomicExch(status, WPC_ERR_BAD_ARGUMENT);
     } else {
-      from = (((size_t)layer * n_pages + sp) * nkv + g) * WPC_PAGE + src % WPC_PAGE;
-      to = (((size_t)layer * n_pages + dp) * nkv + g) * WPC_PAGE + i % WPC_PAGE;
-      weight_sums[to] = weight_sums[from];
-      stored_positions[to] = stored_positions[from];
+      from = (((long)layer * n_pages + sp) * nkv + g) * WPC_PAGE + src % WPC_PAGE;
+      to = (((long)layer * n_pages + dp) * nkv + g) * WPC_PAGE + i % WPC_PAGE;
     }
   }
-  for (uint32_t left = __ballot_sync(0xffffffffu, moves); left; left &= left - 1) {
-    const int l = __ffs(left) - 1;
-    const size_t f = __shfl_sync(0xffffffffu, from, l), t = __shfl_sync(0xffffffffu, to, l);
-    for (int e = lane * (int)sizeof(V); e < k_bytes; e += 32 * (int)sizeof(V))
-      *(V*)(k_pages + t * k_bytes + e) = *(const V*)(k_pages + f * k_bytes + e);
-    for (int e = lane * (int)sizeof(V); e < v_bytes; e += 32 * (int)sizeof(V))
-      *(V*)(v_pages + t * v_bytes + e) = *(const V*)(v_pages + f * v_bytes + e);
+  __syncthreads();
+  const uint32_t who = __ballot_sync(0xffffffffu, moves);
+  int first = 0;
+  if (lane == 0 && who) first = atomicAdd(&s_n, __popc(who));               // (the order of the moves does not matter)
+  first = __shfl_sync(0xffffffffu, first, 0);
+  if (moves) {
+    const int at = first + __popc(who & ((1u << lane) - 1));
+    s_from[at] = from;
+    s_to[at] = to;
+    weight_sums[to] = weight_sums[from];
+    stored_positions[to] = stored_positions[from];
+  }
+  __syncthreads();
+  const int chunks = k_chunks + v_chunks, all = s_n * chunks;
+  for (int c0 = tid; c0 < all; c0 += MOVE_THREADS * MOVE_DEPTH) {
+    V v[MOVE_DEPTH];
+    V* dst[MOVE_DEPTH];
+#pragma unroll
+    for (int j = 0; j < MOVE_DEPTH; ++j) {
+      const int c = c0 + j * MOVE_THREADS;
+      dst[j] = nullptr;
+      if (c < all) {
+        const int m = c / chunks, in = c - m * chunks;
+        const bool key = in < k_chunks;
+        const V* from_p = key ? k_pages + s_from[m] * k_chunks + in : v_pages + s_from[m] * v_chunks + (in - k_chunks);
+        dst[j] = key ? k_pages + s_to[m] * k_chunks + in : v_pages + s_to[m] * v_chunks + (in - k_chunks);
+        v[j] = *from_p;
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < MOVE_DEPTH; ++j)
+      if (dst[j]) *dst[j] = v[j];
   }
 }
 
@@ -207,21 +369,32 @@ int wpc_select_kept(const float* weight_sums, const int* stored_positions, const
   if (layers <= 0 || B <= 0 || nkv <= 0) return 0;
   if (keep < 1 || sinks < 0 || recent < 0 || sinks > keep - recent || n_pages < 1 || table_width < 0) return WPC_ERR_BAD_ARGUMENT;
   if (layers > 65535 || B > 65535) return WPC_ERR_UNSUPPORTED;
-  const long holes = (long)keep * 4, keys = (long)table_width * WPC_PAGE * 4, most = 200 * 1024;
-  if (holes > most) return WPC_ERR_TOO_LARGE;
+  const long n = (long)table_width * WPC_PAGE, most = 200 * 1024;
+  const int places = keep < n ? keep : 0;               // (a table that holds no more loses nothing)
+  if ((long)places * 4 > most) return WPC_ERR_TOO_LARGE;
+  const bool wide = (((uintptr_t)weight_sums | (uintptr_t)stored_positions) & 15) == 0;
   const dim3 grid(nkv, B, layers);
   const size_t layer_stride = (size_t)n_pages * nkv * WPC_PAGE;
-  if (holes + keys <= most) {
+  // A thread's share of the keys stays in registers as long as a block of 1,024 threads holds them all
+  // (and the records can be read 16 bytes a load).
+#define WPC_SELECT(NT, ITEMS)                                                                                        \
+  do {                                                                                                               \
+    static int configured[MAX_DEVICES];                                                                              \
+    if (int rc = allow_smem(select_kept_kernel<NT, ITEMS>, places * 8, configured)) return rc;                       \
+    wpc::launch(select_kept_kernel<NT, ITEMS>, grid, NT, places * 8, stream, weight_sums, stored_positions,          \
+                layer_stride, page_table, table_width, lens, next_positions, nkv, n_pages, keep, sinks, recent, kept, \
+                status);                                                                                             \
+  } while (0)
+  if (wide && n <= 512 * 8) WPC_SELECT(512, 8);
+  else if (wide && n <= 1024 * 8) WPC_SELECT(1024, 8);
+  else if (wide && n <= 1024 * 32 && places <= 24 * 1024) WPC_SELECT(1024, 32);
+  else {
     static int configured[MAX_DEVICES];
-    if (int rc = allow_smem(select_kept_kernel<true>, (int)(holes + keys), configured)) return rc;
-    wpc::launch(select_kept_kernel<true>, grid, SEL_THREADS, holes + keys, stream, weight_sums, stored_positions, layer_stride,
-                page_table, table_width, lens, next_positions, nkv, n_pages, keep, sinks, recent, kept, status);
-  } else {
-    static int configured[MAX_DEVICES];
-    if (int rc = allow_smem(select_kept_kernel<false>, (int)holes, configured)) return rc;
-    wpc::launch(select_kept_kernel<false>, grid, SEL_THREADS, holes, stream, weight_sums, stored_positions, layer_stride,
+    if (int rc = allow_smem(select_kept_long_kernel, places * 4, configured)) return rc;
+    wpc::launch(select_kept_long_kernel, grid, SEL_THREADS, places * 4, stream, weight_sums, stored_positions, layer_stride,
                 page_table, table_width, lens, next_positions, nkv, n_pages, keep, sinks, recent, kept, status);
   }
+#undef WPC_SELECT
   return launch_status();
 }
 
@@ -231,15 +404,15 @@ int wpc_move_kept(void* k_pages, void* v_pages, int k_bytes, int v_bytes, float*
   if (layers <= 0 || B <= 0 || nkv <= 0 || keep <= 0) return 0;
   const long rows = (long)layers * B * nkv;
   if (rows > 65535) return WPC_ERR_TOO_LARGE;
-  const dim3 grid((keep + MOVE_THREADS - 1) / MOVE_THREADS, (unsigned)rows);
+  const dim3 grid((keep + MOVE_PLACES - 1) / MOVE_PLACES, (unsigned)rows);
   const uintptr_t align = (uintptr_t)k_pages | (uintptr_t)v_pages | (uintptr_t)k_bytes | (uintptr_t)v_bytes;
-  auto go = [&](auto kernel) {
-    wpc::launch(kernel, grid, MOVE_THREADS, 0, stream, (uint8_t*)k_pages, (uint8_t*)v_pages, k_bytes, v_bytes, weight_sums,
+  auto go = [&](auto kernel, auto* k, auto* v) {
+    wpc::launch(kernel, grid, MOVE_THREADS, 0, stream, k, v, k_bytes / (int)sizeof(*k), v_bytes / (int)sizeof(*v), weight_sums,
                 stored_positions, page_table, table_width, kept, B, nkv, n_pages, keep, status);
   };
-  if (align % 16 == 0) go(move_kept_kernel<uint4>);
-  else if (align % 4 == 0) go(move_kept_kernel<uint32_t>);
-  else if (align % 2 == 0) go(move_kept_kernel<uint16_t>);
+  if (align % 16 == 0) go(move_kept_kernel<uint4>, (uint4*)k_pages, (uint4*)v_pages);
+  else if (align % 4 == 0) go(move_kept_kernel<uint32_t>, (uint32_t*)k_pages, (uint32_t*)v_pages);
+  else if (align % 2 == 0) go(move_kept_kernel<uint16_t>, (uint16_t*)k_pages, (uint16_t*)v_pages);
   else return WPC_ERR_UNSUPPORTED;
   pdl_skip_next() = 1;      // (the kernel behind starts when the moves are done and visible)
   return launch_status();
