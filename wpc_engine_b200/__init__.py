@@ -10,13 +10,13 @@ feed-forward, block), models/ (a decoder as data, and the Qwen2 builder), cache/
 per-sequence state), engine/ (the step function and the generation loop), sampling/, ops.py
 (the Python face of the kernels) and csrc/ (the CUDA sources and their in-tree build).
 """
-from .cache import CacheError
+from .cache import CacheError, CacheEviction
 from .config import ConfigError, Qwen2Config
 from .engine import Engine, GenerationOptions, SequenceStep, generate
 from .ops import KernelError
 from .registry import architecture_names, register_architecture, resolve, unregister_architecture
 from .weights import WeightError, write_random_model
 
-__all__ = ["CacheError", "ConfigError", "Engine", "GenerationOptions", "KernelError", "Qwen2Config",
-           "SequenceStep", "WeightError", "architecture_names", "generate", "register_architecture",
+__all__ = ["CacheError", "CacheEviction", "ConfigError", "Engine", "GenerationOptions", "KernelError",
+           "Qwen2Config", "SequenceStep", "WeightError", "architecture_names", "generate", "register_architecture",
            "resolve", "unregister_architecture", "write_random_model"]

@@ -4,8 +4,11 @@ and per-sequence records of fixed size.
 Storage is grouped by what the layers need (`KVSpec` with or without a window, `StateSpec`):
 every group has tensors and a page pool of its own.  A sequence holds, in each key/value
 group, the pages that cover its positions; in a group with a window the pages that lie wholly
-before the window are given back after every step.  Position p of a sequence lives in page
-`table[p // PAGE]` at row `p % PAGE`.
+before the window are given back after every step, but for those of its sinks.  Position p of a
+sequence lives in page `table[p // PAGE]` at row `p % PAGE`.  With `CacheEviction` the groups without
+a window hold a bounded number of entries of each sequence: an entry's place is then no
+longer its position, and the group records for every layer, KV head and place the position and the
+attention weight that the entry has received.
 
 The reference keeps one growable vector per layer and KV head for its single sequence
 (wpc-runtime/src/model.rs:38-62); slots, pages and groups have no counterpart there.
@@ -19,6 +22,7 @@ import torch
 
 from ..constants import PAGE          # positions per page; `--max-tokens` is counted in these units
 from ..parts.base import KVSpec, StateSpec
+from .eviction import CacheEviction
 from .pages import CacheError, FreeList
 
 
@@ -33,6 +37,11 @@ class KVView:
     v_pages: torch.Tensor        # [n_pages, n_kv_heads, PAGE, value_dim]
     page_table: torch.Tensor     # int32 [B, width]: page of block i of sequence b, -1 if none
     writes: bool = True
+    # of a cache that entries are taken out of (CacheEviction), else None:
+    places: Optional[torch.Tensor] = None            # int32 [T] where this step's tokens are stored
+    stored_lens: Optional[torch.Tensor] = None       # int32 [B] entries that a sequence holds after this step
+    weight_sums: Optional[torch.Tensor] = None       # float32 [n_pages, n_kv_heads, PAGE] weight received so far
+    stored_positions: Optional[torch.Tensor] = None  # int32, the same shape: position of each entry
 
 
 @dataclass
@@ -43,26 +52,32 @@ class StateView:
     writes: bool = True
 
 
-def window_pages(window: int, max_step_tokens: int) -> int:
+def window_pages(window: int, max_step_tokens: int, sinks: int = 0) -> int:
     """The most pages that one sequence holds in a group with `window` when no step brings it
     more than max_step_tokens tokens: the blocks from the first position that the step's first
-    query sees to the step's last position."""
-    return pages_for(window + max_step_tokens - 1) + 1
+    query sees to the step's last position, and those of the sinks."""
+    return pages_for(window + max_step_tokens - 1) + 1 + pages_for(sinks)
 
 
 class KVGroup:
     """The keys and values of the cache layers that share one `KVSpec`: tensors and a page pool of
     the group's own.  `pages_per_sequence` (windowed groups of an engine whose steps are bounded)
-    is the most pages that one sequence ever holds here, None where its length alone bounds it."""
+    is the most pages that one sequence ever holds here, None where its length alone bounds it.
+    `evicts`: entries are taken out (`CacheEviction`), so the group keeps their records."""
 
     def __init__(self, spec: KVSpec, n_layers: int, n_pages: int, dtype: torch.dtype, device,
-                 pages_per_sequence: Optional[int] = None):
+                 pages_per_sequence: Optional[int] = None, evicts: bool = False):
         self.spec = spec
         self.n_layers = n_layers
         self.n_pages = n_pages
         self.pages_per_sequence = pages_per_sequence
         self.k = torch.zeros((n_layers, n_pages, spec.n_kv_heads, PAGE, spec.head_dim), dtype=dtype, device=device)
         self.v = torch.zeros((n_layers, n_pages, spec.n_kv_heads, PAGE, spec.value_dim), dtype=dtype, device=device)
+        self.evicts = bool(evicts)
+        if self.evicts:
+            record = (n_layers, n_pages, spec.n_kv_heads, PAGE)
+            self.weight_sums = torch.zeros(record, dtype=torch.float32, device=device)
+            self.stored_positions = torch.zeros(record, dtype=torch.int32, device=device)
         self.pool = FreeList(n_pages, "page")
         self.tables: Dict[int, List[int]] = {}        # slot -> page of each block (-1: given back)
 
@@ -95,7 +110,7 @@ class KVGroup:
             return
         first_visible = max(0, length - self.spec.window + 1)   # of the next query, at `length`
         table = self.tables[slot]
-        for block in range(first_visible // PAGE):
+        for block in range(pages_for(self.spec.sinks), first_visible // PAGE):
             if table[block] >= 0:
                 self.pool.give_back(table[block])
                 table[block] = -1
@@ -124,12 +139,15 @@ class SequenceCache:
     up to whole pages.  It sizes the pool of every key/value group that keeps all positions.
     A group with a window needs less when no step brings a sequence more than `max_step_tokens`
     tokens (None: unbounded): then each of the `max_sequences` slots holds at most
-    `window_pages(window, max_step_tokens)` pages there, and the pool is that small.  A model
+    `window_pages(window, max_step_tokens, sinks)` pages there, and the pool is that small.  With
+    `eviction` the groups without a window are bounded in the same way: a slot holds at most
+    keep + slack entries between steps (`stored`), `cut` takes it back to keep.  A model
     without key/value groups has no pages at all.
     """
 
     def __init__(self, cache_specs: Sequence[object], max_tokens: int, dtype: torch.dtype, device,
-                 max_sequences: Optional[int] = None, max_step_tokens: Optional[int] = None):
+                 max_sequences: Optional[int] = None, max_step_tokens: Optional[int] = None,
+                 eviction: Optional[CacheEviction] = None):
         self.device = device
         self.n_pages = pages_for(max_tokens)
         if self.n_pages < 1:
@@ -138,6 +156,8 @@ class SequenceCache:
         self.max_step_tokens = None if max_step_tokens is None else int(max_step_tokens)
         self.slots = FreeList(self.n_slots, "slot")
         self.lengths: Dict[int, int] = {}
+        self.eviction = eviction
+        self.stored: Dict[int, int] = {}                 # entries in the groups that evict (lengths without eviction)
         self.groups: List[object] = []
         self.layer_group: List[Optional[int]] = []       # cache layer -> group
         self.layer_index: List[Optional[int]] = []       # cache layer -> layer within the group
@@ -151,9 +171,13 @@ class SequenceCache:
             if isinstance(spec, KVSpec):
                 per_seq, n_pages = None, self.n_pages
                 if spec.window is not None and self.max_step_tokens is not None:
-                    per_seq = window_pages(spec.window, self.max_step_tokens)
+                    per_seq = window_pages(spec.window, self.max_step_tokens, spec.sinks)
+                evicts = eviction is not None and spec.window is None
+                if evicts and self.max_step_tokens is not None:
+                    per_seq = pages_for(eviction.keep + eviction.slack + self.max_step_tokens)
+                if per_seq is not None:
                     n_pages = min(self.n_pages, self.n_slots * per_seq)
-                group = KVGroup(spec, len(layers), n_pages, dtype, device, per_seq)
+                group = KVGroup(spec, len(layers), n_pages, dtype, device, per_seq, evicts)
             elif isinstance(spec, StateSpec):
                 group = StateGroup(spec, len(layers), self.n_slots, device)
             else:
@@ -169,7 +193,7 @@ class SequenceCache:
     # -- slots -----------------------------------------------------------------------------
     def open(self) -> int:
         slot = self.slots.take()
-        self.lengths[slot] = 0
+        self.lengths[slot] = self.stored[slot] = 0
         for g in self.groups:
             g.open(slot)
         return slot
@@ -180,7 +204,7 @@ class SequenceCache:
         for g in self.groups:
             if isinstance(g, KVGroup):
                 g.close(slot)
-        del self.lengths[slot]
+        del self.lengths[slot], self.stored[slot]
         self.slots.give_back(slot)
 
     def length(self, slot: int) -> int:
@@ -192,14 +216,14 @@ class SequenceCache:
         start = self.lengths[slot]
         for g in self.groups:
             if isinstance(g, KVGroup):
-                g.reserve(slot, start + n_new)
+                g.reserve(slot, (self.stored[slot] if g.evicts else start) + n_new)
         return start
 
     def release_unused(self, slot: int) -> None:
         """Undoes `reserve` for a step that did not run: pages behind the sequence's length go back."""
         for g in self.groups:
             if isinstance(g, KVGroup):
-                g.release_beyond(slot, self.lengths[slot])
+                g.release_beyond(slot, self.stored[slot] if g.evicts else self.lengths[slot])
 
     def fits(self, token_counts: Sequence[int]) -> bool:
         """Whether sequences grown to these many positions can all live in the cache at once."""
@@ -212,9 +236,26 @@ class SequenceCache:
 
     def commit(self, slot: int, n_new: int) -> None:
         self.lengths[slot] += n_new
+        self.stored[slot] += n_new
         for g in self.groups:
             if isinstance(g, KVGroup):
                 g.trim(slot, self.lengths[slot])
+
+    # -- eviction ----------------------------------------------------------------------------
+    def evicting_groups(self) -> List[int]:
+        return [i for i, g in enumerate(self.groups) if isinstance(g, KVGroup) and g.evicts]
+
+    def over(self, slots: Sequence[int]) -> List[int]:
+        """Those of the slots that hold more entries than they may between steps."""
+        e = self.eviction
+        return [] if e is None else [s for s in slots if self.stored[s] > e.keep + e.slack]
+
+    def cut(self, slot: int) -> None:
+        """The first `keep` places hold what stays: the pages behind them go back."""
+        self.stored[slot] = min(self.stored[slot], self.eviction.keep)
+        for g in self.groups:
+            if isinstance(g, KVGroup) and g.evicts:
+                g.release_beyond(slot, self.stored[slot])
 
     def table_width(self, slots: Sequence[int]) -> int:
         width = 1

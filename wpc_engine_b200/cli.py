@@ -4,7 +4,8 @@ they mean there.  The reference tokenizes `--prompt TEXT`; this library takes to
 the prompt is `--prompt-ids "1,2,3;4,5"` (`;` separates the requests of a batch).  Added:
 `--temperature`, `--seed`, `--stop-ids`, `--dtype`, `--random-weights` (with `--config FILE`,
 writes a model folder into `--model` first), `--max-seq-len`, `--print-logits K`, `--max-batch`,
-`--cache-tokens`.  `--arch` names the architecture or `auto`
+`--cache-tokens`, `--max-step-tokens`, and `--cache-keep` with `--cache-recent` and `--cache-sinks`.
+`--arch` names the architecture or `auto`
 (config.json decides, main.rs:69-82).  Standard output carries one JSON line per request;
 diagnostics go to standard error in the reference's wording (main.rs:100-104, 294, 309, 424,
 429).
@@ -44,6 +45,13 @@ def build_parser() -> argparse.ArgumentParser:
     ap.add_argument("--config", help="config.json for --random-weights")
     ap.add_argument("--max-batch", type=int, default=None)
     ap.add_argument("--cache-tokens", type=int, default=None, help="positions the cache holds (default: what fits the prompts)")
+    ap.add_argument("--max-step-tokens", type=int, default=None, help="feed prompts in chunks of that many tokens")
+    ap.add_argument("--cache-keep", type=int, default=None,
+                    help="entries that a sequence keeps in layers without a window: the first, the last, and those with "
+                         "the most attention weight (default: all)")
+    ap.add_argument("--cache-recent", type=int, default=None,
+                    help="last positions that --cache-keep always holds (default: a quarter of it)")
+    ap.add_argument("--cache-sinks", type=int, default=4, help="first positions that --cache-keep always holds")
     ap.add_argument("--max-seq-len", type=int, default=None,
                     help="longest sequence (prompt plus generated tokens) that is accepted; default: the model's "
                          "max_position_embeddings")
@@ -56,7 +64,7 @@ def main(argv=None) -> int:
     args = build_parser().parse_args(argv)
     import torch
     from . import Engine, GenerationOptions, generate, write_random_model
-    from .cache import PAGE
+    from .cache import PAGE, CacheEviction
     from .config import read_config_json
     from .registry import resolve
     from .sampling import banned_from_env, stop_ids_of_folder
@@ -80,6 +88,15 @@ def main(argv=None) -> int:
         write_random_model(args.model, cfg, args.seed, torch.bfloat16 if dtype == "bfloat16" else torch.float32)
         print(f"wrote random weights (seed {args.seed}) to {args.model}", file=sys.stderr)
 
+    eviction = None
+    if args.cache_keep is not None:
+        recent = args.cache_keep // 4 if args.cache_recent is None else args.cache_recent
+        try:
+            eviction = CacheEviction(args.cache_keep, recent, args.cache_sinks)
+        except ValueError as e:
+            print(f"error: {e}", file=sys.stderr)
+            return 2
+
     if args.max_seq_len is not None:
         for i, p in enumerate(prompts):
             if len(p) + args.max_tokens > args.max_seq_len:
@@ -96,7 +113,8 @@ def main(argv=None) -> int:
     need = sum((len(p) + args.max_tokens + PAGE - 1) // PAGE * PAGE for p in prompts)
     if args.max_batch:
         need = max((len(p) + args.max_tokens + PAGE - 1) // PAGE * PAGE for p in prompts) * args.max_batch
-    engine = Engine.from_folder(args.model, dtype=dtype, device="cuda", max_tokens=args.cache_tokens or need)
+    engine = Engine.from_folder(args.model, dtype=dtype, device="cuda", max_tokens=args.cache_tokens or need,
+                                max_step_tokens=args.max_step_tokens, eviction=eviction)
     c = engine.config
     print(f"config: hidden={c.hidden_size} layers={c.num_hidden_layers} heads={c.num_attention_heads} "
           f"kv_heads={c.num_key_value_heads} vocab={c.vocab_size}", file=sys.stderr)

@@ -7,6 +7,8 @@ and `head_dim` to hidden_size / num_attention_heads (config.rs:59-62).  The wind
 are not read by the reference; here they mean what their names say: with
 `use_sliding_window` set, layers `max_window_layers` and above see only the last
 `sliding_window` positions, and no sequence may grow beyond `max_position_embeddings`.
+`attention_sinks` (no key of the published models): how many of the first positions those
+layers see beside their window.
 """
 from __future__ import annotations
 
@@ -33,6 +35,7 @@ class Qwen2Config:
     sliding_window: Optional[int] = None
     use_sliding_window: bool = False
     max_window_layers: Optional[int] = None
+    attention_sinks: Optional[int] = None
     eos_token_id: Any = None          # a number or a list of numbers (main.rs:449-488)
     bos_token_id: Optional[int] = None
     model_type: Optional[str] = None
@@ -66,6 +69,8 @@ class Qwen2Config:
             require_int("sliding_window", self.sliding_window)
         if self.max_window_layers is not None:
             require_int("max_window_layers", self.max_window_layers, minimum=0)
+        if self.attention_sinks is not None:
+            require_int("attention_sinks", self.attention_sinks, minimum=0)
         if self.use_sliding_window:
             require(self.sliding_window is not None, "use_sliding_window is set but sliding_window is not given")
         eos = self.eos_token_id
@@ -94,6 +99,10 @@ class Qwen2Config:
         if not self.use_sliding_window or self.sliding_window is None:
             return None
         return self.sliding_window if layer >= (self.max_window_layers or 0) else None
+
+    def sinks_of_layer(self, layer: int) -> int:
+        """First positions that `layer` sees beside its window."""
+        return 0 if self.window_of_layer(layer) is None else self.attention_sinks or 0
 
     # -- reading and writing -----------------------------------------------------------------
     @classmethod

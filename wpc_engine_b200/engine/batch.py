@@ -29,6 +29,7 @@ class StepLayout:
     n_want: int
     table_width: int
     n_kv_groups: int
+    eviction: bool = False            # places and stored lengths differ from positions and lengths
     tokens: int = 0
     positions: int = 0
     seq_of_token: int = 0
@@ -37,6 +38,8 @@ class StepLayout:
     slots: int = 0
     want_rows: int = 0
     tables: int = 0
+    places: int = 0
+    stored_lens: int = 0
     total: int = 0
 
     def __post_init__(self):
@@ -51,6 +54,9 @@ class StepLayout:
         self.slots = off; off = align(off + self.n_seqs)
         self.want_rows = off; off = align(off + max(self.n_want, 1))
         self.tables = off; off = align(off + self.n_kv_groups * self.n_seqs * self.table_width)
+        if self.eviction:
+            self.places = off; off = align(off + self.n_tokens)
+            self.stored_lens = off; off = align(off + self.n_seqs)
         self.total = off
 
 
@@ -62,13 +68,15 @@ class StepPlan:
     max_ctx_len: int
     is_decode: bool
     starts: List[int]                 # position of each sequence's first new token
+    max_stored_len: int = 0           # most entries that a sequence holds after the step (with eviction)
 
 
 def plan_step(entries: Sequence[SequenceStep], starts: Sequence[int],
               table_rows: Sequence[Sequence[Sequence[int]]], table_width: int,
-              out: Optional[np.ndarray] = None) -> StepPlan:
+              out: Optional[np.ndarray] = None, stored: Optional[Sequence[int]] = None) -> StepPlan:
     """starts[b]: the length of sequence b before this step.  table_rows[g][b]: the page table
-    row (already `table_width` wide) of sequence b in key/value group g."""
+    row (already `table_width` wide) of sequence b in key/value group g.  stored[b], for a cache that
+    entries are taken out of: how many it holds of sequence b before this step."""
     n_seqs = len(entries)
     if n_seqs == 0:
         raise ValueError("a step needs at least one sequence")
@@ -77,7 +85,7 @@ def plan_step(entries: Sequence[SequenceStep], starts: Sequence[int],
         raise ValueError("every sequence of a step brings at least one token")
     n_tokens = sum(lens)
     n_want = sum(len(e.want) for e in entries)
-    lay = StepLayout(n_tokens, n_seqs, n_want, table_width, len(table_rows))
+    lay = StepLayout(n_tokens, n_seqs, n_want, table_width, len(table_rows), stored is not None)
     host = out[: lay.total] if out is not None else np.empty(lay.total, dtype=np.int32)
     host[:] = 0
     t = 0
@@ -89,6 +97,9 @@ def plan_step(entries: Sequence[SequenceStep], starts: Sequence[int],
         host[lay.seq_of_token + t: lay.seq_of_token + t + n] = b
         host[lay.cu_seqlens + b] = t
         host[lay.ctx_lens + b] = starts[b] + n
+        if stored is not None:
+            host[lay.places + t: lay.places + t + n] = np.arange(stored[b], stored[b] + n)
+            host[lay.stored_lens + b] = stored[b] + n
         host[lay.slots + b] = e.slot
         for place in e.want:
             if not 0 <= place < n:
@@ -101,7 +112,8 @@ def plan_step(entries: Sequence[SequenceStep], starts: Sequence[int],
         base = lay.tables + g * n_seqs * table_width
         host[base: base + n_seqs * table_width] = np.asarray(rows, dtype=np.int32).reshape(-1)
     return StepPlan(lay, host, max(lens), max(s + n for s, n in zip(starts, lens)),
-                    all(n == 1 for n in lens), list(starts))
+                    all(n == 1 for n in lens), list(starts),
+                    0 if stored is None else max(s + n for s, n in zip(stored, lens)))
 
 
 @dataclass
@@ -121,12 +133,16 @@ class StepContext:
     max_new_tokens: int
     max_ctx_len: int
     is_decode: bool
+    places: Optional[torch.Tensor] = None          # int32 [T] where tokens are stored, in groups that evict
+    stored_lens: Optional[torch.Tensor] = None     # int32 [B] entries of each sequence there, after this step
+    max_stored_len: int = 0
     new_tokens_host: Optional[List[int]] = None   # tokens that each sequence brings, on the host (all 1 in a graph)
     shared: Dict[object, object] = field(default_factory=dict)   # per-step tables of the parts
 
 
 def context_from(meta: torch.Tensor, lay: StepLayout, act_dtype: torch.dtype, max_new_tokens: int,
-                 max_ctx_len: int, is_decode: bool, new_tokens_host: Optional[List[int]] = None) -> StepContext:
+                 max_ctx_len: int, is_decode: bool, new_tokens_host: Optional[List[int]] = None,
+                 max_stored_len: int = 0) -> StepContext:
     def view(off, n):
         return meta[off: off + n]
     tables = []
@@ -139,5 +155,7 @@ def context_from(meta: torch.Tensor, lay: StepLayout, act_dtype: torch.dtype, ma
         seq_of_token=view(lay.seq_of_token, lay.n_tokens),
         cu_seqlens=view(lay.cu_seqlens, lay.n_seqs + 1), ctx_lens=view(lay.ctx_lens, lay.n_seqs),
         slots=view(lay.slots, lay.n_seqs), want_rows=view(lay.want_rows, lay.n_want),
+        places=view(lay.places, lay.n_tokens) if lay.eviction else None,
+        stored_lens=view(lay.stored_lens, lay.n_seqs) if lay.eviction else None, max_stored_len=max_stored_len,
         page_tables=tables, max_new_tokens=max_new_tokens, max_ctx_len=max_ctx_len, is_decode=is_decode,
         new_tokens_host=new_tokens_host if new_tokens_host is not None else ([1] * lay.n_seqs if is_decode else None))

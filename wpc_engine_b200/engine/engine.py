@@ -14,7 +14,7 @@ import numpy as np
 import torch
 
 from .. import ops
-from ..cache import PAGE, CacheError, SequenceCache
+from ..cache import PAGE, CacheError, CacheEviction, SequenceCache
 from ..registry import config_from_folder, resolve
 from ..weights import load_weights, random_weights_on_device
 from .batch import SequenceStep, StepLayout, context_from, plan_step
@@ -77,13 +77,17 @@ class Engine:
     groups that keep a window are sized by the window.  check_status: `step` reads the device
     error word after it has run (which waits for the device) and raises `KernelError` if a
     kernel gave up; callers that keep the device busy pass `check=False` to `step` and read the
-    word with their results (`generate` does).
+    word with their results (`generate` does).  eviction: what the layers without a window keep of a
+    sequence that outgrows it (`CacheEviction`; None: everything).  With `max_step_tokens` the cache is
+    sized by it; without, a step that brings a whole prompt needs pages for all of it until it
+    has run.
 
     The limits of a step come from the model: `model.vocab_size` and `model.max_positions`."""
 
     def __init__(self, model, dtype, device="cuda", max_tokens: int = 4096,
                  max_sequences: Optional[int] = None, use_graphs: bool = True,
-                 max_step_tokens: Optional[int] = None, check_status: bool = True):
+                 max_step_tokens: Optional[int] = None, check_status: bool = True,
+                 eviction: Optional[CacheEviction] = None):
         self.model = model
         self.config = model.config
         self.dtype = parse_dtype(dtype)
@@ -91,8 +95,10 @@ class Engine:
         if max_step_tokens is not None and max_step_tokens < 1:
             raise ValueError(f"max_step_tokens must be at least 1, got {max_step_tokens}")
         self.max_step_tokens = max_step_tokens
+        if eviction is not None and not model.serves_eviction():
+            raise ValueError("a layer of this model cannot serve a cache that entries are taken out of")
         self.cache = SequenceCache(model.cache_specs(), max_tokens, self.dtype, self.device, max_sequences,
-                                   max_step_tokens)
+                                   max_step_tokens, eviction)
         self._ring = _MetaRing(self.device)
         self.use_graphs = bool(use_graphs) and self.device.type == "cuda" and model.graph_safe()
         self.check_status = bool(check_status) and self.device.type == "cuda"
@@ -200,7 +206,45 @@ class Engine:
         for e in entries:
             self.cache.commit(e.slot, len(e.tokens))
         self.steps_run += 1
+        over = self.cache.over([e.slot for e in entries])
+        if over:
+            self._evict(over)
         return logits
+
+    def _evict(self, slots: Sequence[int]) -> None:
+        """Cuts the sequences in `slots` down to what the eviction keeps (queued behind the step; the
+        pages go back at once, since what is queued later runs later)."""
+        e = self.cache.eviction
+        n = len(slots)
+        for i in self.cache.evicting_groups():
+            group = self.cache.groups[i]
+            width = max(len(group.tables[s]) for s in slots)
+            host = self._ring.next(n * (width + 2))
+            block = host.numpy()
+            block[: n] = [self.cache.stored[s] for s in slots]
+            block[n: 2 * n] = [self.cache.length(s) for s in slots]
+            block[2 * n: n * (width + 2)] = np.asarray(self.cache.page_table_rows(i, slots, width), dtype=np.int32).reshape(-1)
+            meta = host[: n * (width + 2)].to(self.device, non_blocking=True)
+            self._ring.sent()
+            table = meta[2 * n:].view(n, width)
+            kept = ops.select_kept(group.weight_sums, group.stored_positions, table, meta[: n], meta[n: 2 * n],
+                                   e.keep, e.sinks, e.recent)
+            ops.move_kept_(group.k, group.v, group.weight_sums, group.stored_positions, table, kept)
+        for s in slots:
+            self.cache.cut(s)
+
+    def stored_positions(self, slot: int) -> List[torch.Tensor]:
+        """The positions whose keys and values a sequence still holds where entries are taken out: for
+        each such group of layers int32 [layers, KV heads, entries], in the order in which they
+        are stored (copied; waits for the device)."""
+        out = []
+        for i in self.cache.evicting_groups():
+            group = self.cache.groups[i]
+            pages = torch.tensor(group.tables[slot], dtype=torch.int64)
+            rows = group.stored_positions[:, pages.to(self.device)]          # [layers, blocks, heads, PAGE]
+            rows = rows.permute(0, 2, 1, 3).reshape(rows.shape[0], rows.shape[2], -1)
+            out.append(rows[..., : self.cache.stored[slot]].contiguous())
+        return out
 
     def _run(self, entries, starts, device_tokens, borrow) -> Optional[torch.Tensor]:
         slots = [e.slot for e in entries]
@@ -209,9 +253,10 @@ class Engine:
         rows = [self.cache.page_table_rows(g, slots, width) for g in kv_groups]
         n_tokens = sum(len(e.tokens) for e in entries)
         n_want = sum(len(e.want) for e in entries)
-        lay = StepLayout(n_tokens, len(entries), n_want, width, len(kv_groups))
+        stored = None if self.cache.eviction is None else [self.cache.stored[s] for s in slots]
+        lay = StepLayout(n_tokens, len(entries), n_want, width, len(kv_groups), stored is not None)
         host = self._ring.next(lay.total)
-        plan = plan_step(entries, starts, rows, width, out=host.numpy())
+        plan = plan_step(entries, starts, rows, width, out=host.numpy(), stored=stored)
         logits = None
         ran = False
         if device_tokens is not None and not (plan.is_decode and device_tokens.numel() == len(entries)
@@ -227,7 +272,7 @@ class Engine:
             if device_tokens is not None:
                 meta[lay.tokens: lay.tokens + lay.n_tokens].copy_(device_tokens)
             ctx = context_from(meta, lay, self.dtype, plan.max_new_tokens, plan.max_ctx_len, plan.is_decode,
-                               [len(e.tokens) for e in entries])
+                               [len(e.tokens) for e in entries], plan.max_stored_len)
             logits = self.model.forward(ctx, self.cache)
         return logits
 
@@ -243,7 +288,8 @@ class Engine:
             return False, None
         if entry == "seen":
             meta = torch.zeros(lay.total, dtype=torch.int32, device=self.device)
-            ctx = context_from(meta, lay, self.dtype, 1, lay.table_width * PAGE, True)
+            ctx = context_from(meta, lay, self.dtype, 1, lay.table_width * PAGE, True,
+                               max_stored_len=lay.table_width * PAGE)
             graph = torch.cuda.CUDAGraph()
             before = ops.launch_count
             with torch.cuda.graph(graph):

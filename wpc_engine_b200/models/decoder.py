@@ -11,7 +11,7 @@ from typing import Dict, List, Optional, Sequence, Tuple
 import torch
 
 from ..cache import KVGroup, KVView, SequenceCache, StateGroup, StateView
-from ..parts.base import Block, Norm, Part, all_graph_safe, collect_params
+from ..parts.base import Block, KVSpec, Norm, Part, all_graph_safe, collect_params
 from ..parts.embedding import Embedding, OutputHead
 
 
@@ -77,6 +77,17 @@ class DecoderModel:
     def graph_safe(self) -> bool:
         return all(all_graph_safe(part) for _, part in self.roots())
 
+    def serves_eviction(self) -> bool:
+        """Whether every layer whose cache keeps all positions can do without some of them."""
+        for run in self.schedule:
+            mixer = self.blocks[run.layer].mixer_of()
+            spec = None if mixer is None else mixer.cache_spec()
+            src = spec if run.cache_of is None else self.blocks[self.schedule[run.cache_of].layer].mixer_of().cache_spec()
+            if isinstance(src, KVSpec) and src.window is None:
+                if not mixer.serves_eviction or getattr(mixer, "window", None) is not None:
+                    return False
+        return True
+
     # -- cache -------------------------------------------------------------------------------
     def cache_specs(self) -> List[object]:
         """What each schedule entry keeps per sequence (None for entries that keep nothing or
@@ -99,8 +110,11 @@ class DecoderModel:
                 continue
             group, j = cache.groups[g], cache.layer_index[src]
             if isinstance(group, KVGroup):
-                views.append(KVView(group.k[j], group.v[j], ctx.page_tables[kv_order.index(g)],
-                                    writes=run.cache_of is None))
+                view = KVView(group.k[j], group.v[j], ctx.page_tables[kv_order.index(g)], writes=run.cache_of is None)
+                if group.evicts:
+                    view.places, view.stored_lens = ctx.places, ctx.stored_lens
+                    view.weight_sums, view.stored_positions = group.weight_sums[j], group.stored_positions[j]
+                views.append(view)
             elif isinstance(group, StateGroup):
                 views.append(StateView(group.state[j], ctx.slots, writes=run.cache_of is None))
         return views

@@ -21,7 +21,8 @@ def build_qwen2(config: Qwen2Config) -> DecoderModel:
         blocks.append(PreNormBlock(
             RMSNorm(c.hidden_size, c.rms_norm_eps),
             GQAAttention(c.hidden_size, c.num_attention_heads, c.num_key_value_heads, c.head_dim,
-                         position=rotary, qkv_bias=True, window=c.window_of_layer(layer)),
+                         position=rotary, qkv_bias=True, window=c.window_of_layer(layer),
+                         sinks=c.sinks_of_layer(layer)),
             RMSNorm(c.hidden_size, c.rms_norm_eps),
             SwiGLU(c.hidden_size, c.intermediate_size)))
     embedding = Embedding(c.vocab_size, c.hidden_size)

@@ -18,7 +18,8 @@ class GQAAttention(Mixer):
     residual stream.
 
     Query head qh reads KV head qh // (n_heads // n_kv_heads) (model.rs:484).  `window`
-    None: a query sees every earlier position and itself; else only the last `window`.
+    None: a query sees every earlier position and itself; else only the last `window` and, beside
+    them, the first `sinks` positions (sinks, which draw weight whatever is asked).
     `scale` None: 1/sqrt(head_dim) (model.rs:477).  `q_norm`, `k_norm`: norms of each head
     of q and of k between projection and position encoding (model.rs:447-462; the Qwen2
     layers have none).  All sizes are parameters.
@@ -33,7 +34,7 @@ class GQAAttention(Mixer):
                  window: Optional[int] = None, scale: Optional[float] = None,
                  names=("q_proj", "k_proj", "v_proj", "o_proj"),
                  q_norm: Optional[HeadNorm] = None, k_norm: Optional[HeadNorm] = None,
-                 norm_names=("q_norm", "k_norm")):
+                 norm_names=("q_norm", "k_norm"), sinks: int = 0):
         if n_heads % n_kv_heads:
             raise ValueError(f"n_heads {n_heads} is not a multiple of n_kv_heads {n_kv_heads}")
         self.width = int(width)
@@ -42,6 +43,9 @@ class GQAAttention(Mixer):
         self.head_dim = int(head_dim)
         self.position = position
         self.window = None if window is None else int(window)
+        if sinks < 0:
+            raise ValueError(f"sinks must not be negative, got {sinks}")
+        self.sinks = int(sinks) if self.window is not None else 0
         self.scale = float(scale) if scale is not None else 1.0 / math.sqrt(self.head_dim)
         self.q_proj = Linear(width, n_heads * head_dim, bias=qkv_bias)
         self.k_proj = Linear(width, n_kv_heads * head_dim, bias=qkv_bias)
@@ -59,8 +63,10 @@ class GQAAttention(Mixer):
                 subs[name] = norm
         return subs
 
+    serves_eviction = True
+
     def cache_spec(self):
-        return KVSpec(self.n_kv_heads, self.head_dim, self.window)
+        return KVSpec(self.n_kv_heads, self.head_dim, self.window, sinks=self.sinks)
 
     def finalize(self):
         self.qkv = fuse_rows([self.q_proj, self.k_proj, self.v_proj])
@@ -80,13 +86,14 @@ class GQAAttention(Mixer):
 
     def forward(self, ctx, h: torch.Tensor, cache, residual: torch.Tensor):
         nh, nkv, hd = self.n_heads, self.n_kv_heads, self.head_dim
+        places = ctx.positions if cache.places is None else cache.places
         if cache.writes and self._fused():
             cos = sin = None
             if self.position is not None:
                 cos, sin = self.position.tables(ctx)
             qkv = ops.linear_qk_rope_kv_store(h, self.qkv.weight, self.qkv.bias, nh, nkv, hd, cos, sin,
                                               cache.k_pages, cache.v_pages, cache.page_table,
-                                              ctx.seq_of_token, ctx.positions)
+                                              ctx.seq_of_token, places)
         else:
             # step by step; a layer that reads another layer's cache computes queries only
             qkv = self.qkv.forward(h) if cache.writes else self.q_proj.forward(h)
@@ -98,9 +105,21 @@ class GQAAttention(Mixer):
                 self.position.rotate(ctx, qkv, nh + nkv if cache.writes else nh, hd)
             if cache.writes:
                 ops.qk_rope_kv_store(qkv, nh, nkv, hd, None, None, cache.k_pages, cache.v_pages, cache.page_table,
-                                     ctx.seq_of_token, ctx.positions)
+                                     ctx.seq_of_token, places)
+        lens, max_len, more = ctx.ctx_lens, ctx.max_ctx_len, {}
+        if self.sinks:
+            more["sinks"] = self.sinks
+        if cache.places is not None:
+            # entries are taken out of this cache: places in it are no positions, and the layer that writes it
+            # keeps the weight that every entry receives
+            if self.window is not None:
+                raise ValueError("a layer with a window cannot read a cache that entries are taken out of")
+            lens, max_len = cache.stored_lens, ctx.max_stored_len
+            if cache.writes:
+                more.update(weight_sums=cache.weight_sums, stored_positions=cache.stored_positions,
+                            token_positions=ctx.positions)
         attn = ops.attention(qkv, nh, nkv, hd, cache.k_pages, cache.v_pages, cache.page_table,
-                             ctx.cu_seqlens, ctx.ctx_lens, ctx.seq_of_token, ctx.positions,
-                             self.scale, self.window, ctx.max_new_tokens, ctx.max_ctx_len)
+                             ctx.cu_seqlens, lens, ctx.seq_of_token, places,
+                             self.scale, self.window, ctx.max_new_tokens, max_len, **more)
         self.o_proj.forward(attn, residual=residual)
         return None

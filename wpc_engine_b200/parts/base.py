@@ -58,12 +58,13 @@ class ParamSpec:
 
 @dataclass(frozen=True)
 class KVSpec:
-    """Keys and values per position: `window` None keeps all of them, else the last `window`.
-    `v_head_dim` None: values are as wide as keys (`head_dim`)."""
+    """Keys and values per position: `window` None keeps all of them, else the last `window` and, beside
+    them, the first `sinks`.  `v_head_dim` None: values are as wide as keys (`head_dim`)."""
     n_kv_heads: int
     head_dim: int
     window: Optional[int] = None
     v_head_dim: Optional[int] = None
+    sinks: int = 0
 
     @property
     def value_dim(self) -> int:
@@ -128,6 +129,11 @@ class PositionEncoding(Part):
 
 
 class Mixer(Part):
+    # Whether the mixer serves a cache that entries are taken out of (`CacheEviction`): it stores keys and
+    # values at the places that its `KVView` names, sees the entries stored there, and adds up the
+    # weight that each of them receives.  The engine refuses eviction for a mixer that does not.
+    serves_eviction = False
+
     def cache_spec(self):
         return None
 
