@@ -573,3 +573,40 @@ def test_starved_sums_return_with_1004_and_the_next_ones_are_right(hd):
     s.attend(weight_sums=sums, stored_positions=stored, token_positions=told)
     s.check_sums(sums, stored, old, want, told)
     assert ops.device_status() == 0
+
+
+@pytest.mark.parametrize("heads", [(14, 2, 64), (28, 4, 128), (5, 1, 64), (40, 8, 128), (2, 2, 64)])
+@pytest.mark.parametrize("lens,new", [([300] * 7, [290] * 7), ([1030, 257, 256, 511, 3], [800, 257, 2, 129, 3]),
+                                      ([2000], [2]), ([64, 700], [2, 600])])
+def test_sums_of_shared_key_tiles(heads, lens, new):
+    """Key tiles whose queries are divided among several CTAs, and CTAs that walk several key tiles."""
+    s = Step(torch.bfloat16, *heads, lens, new, seed=sum(new))
+    old, _ = s.record()
+    # (a second call finds the tickets as the first one left them)
+    runs = []
+    for _ in range(2):
+        sums, stored = s.record()
+        s.attend(weight_sums=sums, stored_positions=stored, token_positions=s.pos)
+        runs.append((sums, stored))
+    assert torch.equal(runs[0][0], runs[1][0])
+    s.check_sums(*runs[1], old, fast_want(s), s.pos)
+
+
+def fast_want(s):
+    """The sums in 64 bits on the GPU, for more queries than the plain loop likes."""
+    nh, nkv, hd = s.heads
+    sums, worst, rep = {}, 0.0, nh // nkv
+    table, cu = s.table.tolist(), s.cu.tolist()
+    for b, n in enumerate(s.lens):
+        at = torch.arange(n, device=DEV)
+        pages = torch.tensor([table[b][i // PAGE] for i in range(n)], device=DEV)
+        pos = torch.arange(n - s.new[b], n, device=DEV)[:, None]
+        for g in range(nkv):
+            k = s.k[pages, g, at % PAGE].double()
+            w = torch.zeros(n, dtype=torch.float64, device=DEV)
+            for h in range(g * rep, (g + 1) * rep):
+                x = s.q[cu[b]:cu[b + 1], h * hd:(h + 1) * hd].double()
+                worst = max(worst, float((x.abs() @ k.abs().t()).max()) * s.scale)
+                w += torch.softmax((x @ k.t() * s.scale).masked_fill(at[None] > pos, -math.inf), 1).sum(0)
+            sums[b, g] = w.cpu()
+    return None, None, worst * (2 * hd + 4) * plain.EPS32, sums, max(s.new) * rep

@@ -136,7 +136,8 @@ int wpc_weight_sums_plain(const void* q, int q_stride, int dtype, const void* k_
 int wpc_weight_sums_tc(const void* q, int q_stride, int n_tokens, const void* k_pages, const int* page_table,
                        int table_width, const int* cu_seqlens, const int* ctx_lens, const int* token_positions,
                        const float* lse, int B, int nh, int nkv, int hd, float scale, int max_new, int max_ctx,
-                       int n_pages, float* weight_sums, int* stored_positions, int* status, cudaStream_t stream);
+                       int n_pages, float* weight_sums, int* stored_positions, int* status, float* part, int* tickets,
+                       int n_tickets, cudaStream_t stream);
 
 // eviction.cu.  kept: int32 [layers][B][nkv][keep], the entry that belongs at each place of the kept
 // part (-1 behind a shorter sequence).  weight_sums, stored_positions: [layers][n_pages][nkv][64].

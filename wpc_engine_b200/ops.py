@@ -720,7 +720,7 @@ _SIGNATURES = {
     "wpc_attention_decode_bounded": "pipippp" "ipiiiifiiiiippp" "ipippii" "pppp",
     "wpc_attention_prefill_bounded": "pipippp" "ippiiiiifiipp",
     "wpc_attention_prefill_tc_bounded": "pipippp" "ippiiiiifiippip",
-    "wpc_weight_sums_tc": "piipp" "ipppp" "iiiifiii" "pppp",
+    "wpc_weight_sums_tc": "piipp" "ipppp" "iiiifiii" "pppppip",
     "wpc_weight_sums_plain": "piipp" "ipppp" "iiiifii" "pppp",
     "wpc_select_kept": "pppipp" "iiiiiii" "ppp",
     "wpc_move_kept": "ppiippp" "ip" "iiiii" "pp",
@@ -795,6 +795,16 @@ def _check_step(q, n_heads, n_kv_heads, head_dim, k_pages, v_pages, page_table, 
 _tickets = {}
 
 
+def _stream_tickets(n, like, index, stream) -> torch.Tensor:
+    """At least n tickets (int32, zero between launches) for a call on this stream."""
+    if torch.cuda.is_current_stream_capturing():
+        return like.new_zeros((n,), dtype=torch.int32)
+    tickets = _tickets.get((index, stream))
+    if tickets is None or tickets.numel() < n:
+        tickets = _tickets[index, stream] = like.new_zeros((max(n, 4096),), dtype=torch.int32)
+    return tickets
+
+
 def _decode_scratch(n_seqs, n_kv_heads, n_heads, head_dim, n_ctas, cluster, groups, q, index, stream):
     """(part_o, part_ml, tickets) of a decode step's split work; zeros for none where no two CTAs share
     a pair through memory.  The parts are this call's own.  The tickets, which are zero between
@@ -809,12 +819,7 @@ def _decode_scratch(n_seqs, n_kv_heads, n_heads, head_dim, n_ctas, cluster, grou
         slots = n_ctas + pairs
         n_o, n_ml = slots * 16 * head_dim, slots * 16 * 2
     part = q.new_empty((n_o + n_ml,), dtype=torch.float32)
-    if torch.cuda.is_current_stream_capturing():
-        tickets = q.new_zeros((pairs,), dtype=torch.int32)
-    else:
-        tickets = _tickets.get((index, stream))
-        if tickets is None or tickets.numel() < pairs:
-            tickets = _tickets[index, stream] = q.new_zeros((max(pairs, 4096),), dtype=torch.int32)
+    tickets = _stream_tickets(pairs, q, index, stream)
     return (part, tickets), part.data_ptr(), part.data_ptr() + 4 * n_o, tickets.data_ptr()
 
 
@@ -880,6 +885,9 @@ def _attention_with_sinks(q, n_heads, n_kv_heads, head_dim, k_pages, v_pages, pa
     return out
 
 
+SUMS_KEYS = 256           # keys of a segment of csrc/attention_sums_tc.cu
+
+
 def _attention_with_sums(q, n_heads, n_kv_heads, head_dim, k_pages, v_pages, page_table, cu_seqlens, ctx_lens,
                          seq_of_token, positions, scale, window, max_new_tokens, max_ctx_len, splits, mma_only,
                          cluster, groups, sinks, weight_sums, stored_positions, token_positions) -> torch.Tensor:
@@ -936,9 +944,12 @@ def _attention_with_sums(q, n_heads, n_kv_heads, head_dim, k_pages, v_pages, pag
         _check("attention_prefill_tc_bounded", _typed_function("wpc_attention_prefill_tc_bounded")(
             *shared, *seqs, B, max_new_tokens, n_heads, n_kv_heads, head_dim, scale, 0, 0, lse.data_ptr(), status, n_pages,
             stream))
+        n_sms = _sms_of.get(index) or sms()
+        part = q.new_empty((2 * n_sms * SUMS_KEYS,), dtype=torch.float32)
+        tickets = _stream_tickets(B * n_kv_heads * -(-max_ctx_len // SUMS_KEYS), q, index, stream)
         _check("weight_sums_tc", _typed_function("wpc_weight_sums_tc")(
             q_ptr, q.stride(0), T, k_ptr, table_ptr, table_width, *seqs, token_positions.data_ptr(), lse.data_ptr(), *sizes,
-            max_new_tokens, max_ctx_len, *target))
+            max_new_tokens, max_ctx_len, *target[:4], part.data_ptr(), tickets.data_ptr(), tickets.numel(), stream))
         return out
     else:
         _check("attention_prefill_bounded", _typed_function("wpc_attention_prefill_bounded")(
