@@ -1,4 +1,5 @@
-"""Compiles the CUDA sources of this folder for sm_100a into one shared library, in-tree.
+"""Compiles the CUDA sources of this folder for sm_100a into one shared library, in-tree, and
+host.cpp, the Python face of some of them, into an extension module beside it.
 
 Objects and the library live in `_build/` beside the sources; a stamp of the sources' contents
 and the flags decides whether anything has to be compiled again, so the first call in a fresh
@@ -20,6 +21,7 @@ from typing import List
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_NAME = "libwpc_kernels.so"
+HOST_NAME = "wpc_host.so"
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ["-O3", "-std=c++17", "-lineinfo", "--expt-relaxed-constexpr", "-Xcompiler", "-fPIC",
               "-Xcompiler", "-fvisibility=default"]
@@ -125,5 +127,46 @@ def library_path(verbose: bool = True) -> str:
     return lib
 
 
+def host_module_path(verbose: bool = True) -> str:
+    """The path of an up-to-date extension module, linked against the kernel library and torch."""
+    import sysconfig
+
+    import torch
+    lib = library_path(verbose)
+    out_dir = os.path.dirname(lib)
+    path, stamp_path = os.path.join(out_dir, HOST_NAME), os.path.join(out_dir, "host_stamp")
+    root = os.path.dirname(torch.__file__)
+    cuda = os.path.dirname(os.path.dirname(os.path.realpath(find_nvcc())))
+    flags = ["-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
+             f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
+    want = "\n".join([_digest(["host.cpp", "api.h"]), torch.__version__, sys.version] + flags)
+    try:
+        with open(stamp_path) as f:
+            if f.read() == want and os.path.exists(path):
+                return path
+    except OSError:
+        pass
+    t0 = time.time()
+    if verbose:
+        _say("compiling host.cpp")
+    tmp = path + f".tmp{os.getpid()}"
+    libs = os.path.join(root, "lib")
+    cmd = ["g++"] + flags + [os.path.join(HERE, "host.cpp"), "-o", tmp, "-I", HERE, "-I", os.path.join(root, "include"),
+           "-I", os.path.join(root, "include", "torch", "csrc", "api", "include"), "-I", os.path.join(cuda, "include"),
+           "-I", sysconfig.get_paths()["include"], "-L", out_dir, f"-l:{LIB_NAME}", "-L", libs, "-lc10", "-lc10_cuda",
+           "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python", "-L", os.path.join(cuda, "lib64"), "-lcudart",
+           "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{libs}"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise BuildError(f"g++ failed on host.cpp:\n{r.stdout}\n{r.stderr}")
+    os.replace(tmp, path)
+    with open(stamp_path, "w") as f:
+        f.write(want)
+    if verbose:
+        _say(f"built {path} in {time.time() - t0:.0f} s")
+    return path
+
+
 if __name__ == "__main__":
     print(library_path())
+    print(host_module_path())

@@ -49,6 +49,30 @@ def library():
     return _lib
 
 
+_host = None
+
+
+def host():
+    """The extension module of the operators that csrc/host.cpp serves (built on first use)."""
+    global _host
+    if _host is None:
+        library()
+        with _lib_lock:
+            if _host is None:
+                import importlib.machinery
+                import importlib.util
+                from .csrc.build import BuildError, host_module_path
+                try:
+                    loader = importlib.machinery.ExtensionFileLoader("wpc_host", host_module_path())
+                    module = importlib.util.module_from_spec(importlib.util.spec_from_loader("wpc_host", loader))
+                    loader.exec_module(module)
+                except (BuildError, OSError, ImportError) as e:
+                    raise KernelError(f"the extension module is not available: {e}") from None
+                module.init(KernelError)
+                _host = module
+    return _host
+
+
 def set_wait_policy(limit_ns: int = 2_000_000_000, starve: bool = False) -> None:
     """How long a kernel waits on one of its barriers before it gives up and records an error
     in the device status word (2 s by default).  `starve` is for tests of that path: kernels
@@ -652,17 +676,21 @@ def attention(q: torch.Tensor, n_heads: int, n_kv_heads: int, head_dim: int, k_p
     (int32 [T]).  `positions` are places in the cache here, `token_positions` those in the text:
     they differ once entries have been taken out (`select_kept`).  No page may belong to two
     sequences of the step."""
-    if weight_sums is not None or stored_positions is not None or token_positions is not None:
-        return _attention_with_sums(q, n_heads, n_kv_heads, head_dim, k_pages, v_pages, page_table, cu_seqlens, ctx_lens,
-                                    seq_of_token, positions, scale, window, max_new_tokens, max_ctx_len, splits,
-                                    mma_only, cluster, groups, sinks, weight_sums, stored_positions, token_positions)
-    if sinks:
+    sums = weight_sums is not None or stored_positions is not None or token_positions is not None
+    if sums:
+        if weight_sums is None or stored_positions is None or token_positions is None:
+            raise KernelError("weight_sums, stored_positions and token_positions come together")
+        if window or sinks:
+            raise KernelError("weights are summed over a cache that keeps everything: no window, no sinks")
+    elif sinks:
         if sinks < 0:
             raise KernelError(f"sinks must not be negative, got {sinks}")
-        if window:
-            return _attention_with_sinks(q, n_heads, n_kv_heads, head_dim, k_pages, v_pages, page_table, cu_seqlens,
-                                         ctx_lens, seq_of_token, positions, scale, window, max_new_tokens, max_ctx_len,
-                                         splits, mma_only, cluster, groups, sinks)
+        if window and window < 0:
+            raise KernelError(f"window must be positive, got {window}")
+    if sums or (sinks and window):
+        return _bounded_attention(q, n_heads, n_kv_heads, head_dim, k_pages, v_pages, page_table, cu_seqlens, ctx_lens,
+                                  seq_of_token, positions, scale, window, max_new_tokens, max_ctx_len, splits, mma_only,
+                                  cluster, groups, sinks, weight_sums, stored_positions, token_positions)
     if q.dtype != torch.bfloat16 or not library().wpc_attention_mma_supports(n_heads, n_kv_heads, head_dim):
         return attention_plain(q, n_heads, n_kv_heads, head_dim, k_pages, v_pages, page_table, seq_of_token,
                                positions, scale, window, max_ctx_len)
@@ -715,114 +743,6 @@ def attention(q: torch.Tensor, n_heads: int, n_kv_heads: int, head_dim: int, k_p
     return out
 
 
-# The arguments of the entry points below, told to ctypes once: p an address, i an int, f a float.
-_SIGNATURES = {
-    "wpc_attention_decode_bounded": "pipippp" "ipiiiifiiiiippp" "ipippii" "pppp",
-    "wpc_attention_prefill_bounded": "pipippp" "ippiiiiifiipp",
-    "wpc_attention_prefill_tc_bounded": "pipippp" "ippiiiiifiippip",
-    "wpc_weight_sums_tc": "piipp" "ipppp" "iiiifiii" "pppppip",
-    "wpc_weight_sums_plain": "piipp" "ipppp" "iiiifii" "pppp",
-    "wpc_select_kept": "pppipp" "iiiiiii" "ppp",
-    "wpc_move_kept": "ppiippp" "ip" "iiiii" "pp",
-}
-_typed = {}
-
-
-def _typed_function(name: str):
-    """An entry point with its argument types set: addresses and sizes then pass as plain numbers."""
-    fn = _typed.get(name)
-    if fn is None:
-        types = {"p": ctypes.c_void_p, "i": ctypes.c_int, "f": ctypes.c_float}
-        fn = getattr(library(), name)
-        fn.argtypes = [types[c] for c in _SIGNATURES[name]]
-        _typed[name] = fn
-    return fn
-
-
-def _raw_stream(index: int) -> int:
-    """The handle of the current stream of device `index`."""
-    return torch._C._cuda_getCurrentRawStream(index)
-
-
-def _on_current_device(t: torch.Tensor, name: str) -> int:
-    _need(t.is_cuda, f"{name} must be on a CUDA device")
-    index, current = t.get_device(), torch.cuda.current_device()
-    if index != current:
-        raise KernelError(f"the tensors lie on cuda:{index}, but the current device is cuda:{current}")
-    return index
-
-
-def _is(t: torch.Tensor, dtype: torch.dtype, numel: int, index: int) -> bool:
-    return t.dtype is dtype and t.numel() == numel and t.get_device() == index and t.is_contiguous()
-
-
-def _check_step(q, n_heads, n_kv_heads, head_dim, k_pages, v_pages, page_table, cu_seqlens, ctx_lens, seq_of_token,
-                positions, max_new_tokens, max_ctx_len, single) -> int:
-    """Checks the arguments that all attention of a step over the paged cache shares; returns the
-    device's index.  (A step of one token is hardly longer than this function: messages are made only
-    when they are needed, and where every sequence brings one token, `single`, what a kernel of
-    such a step does not read is not looked at.)"""
-    index = _on_current_device(q, "q")
-    T, B = q.shape[0], ctx_lens.numel()
-    if q.dim() != 2 or q.stride(1) != 1 or q.shape[1] < n_heads * head_dim:
-        raise KernelError("q must be a matrix with unit column stride, at least n_heads * head_dim wide")
-    if n_kv_heads < 1 or n_heads % n_kv_heads:
-        raise KernelError("n_heads must be a multiple of n_kv_heads")
-    shape, dtype = k_pages.shape, q.dtype
-    if not (len(shape) == 4 and shape[1] == n_kv_heads and shape[2] == PAGE and shape[3] == head_dim
-            and v_pages.shape == shape and k_pages.dtype is dtype and v_pages.dtype is dtype
-            and k_pages.is_contiguous() and v_pages.is_contiguous()
-            and k_pages.get_device() == index and v_pages.get_device() == index
-            and (k_pages.data_ptr() | v_pages.data_ptr()) & 15 == 0):
-        raise KernelError("pages must be contiguous [n_pages, n_kv_heads, PAGE, head_dim] of q's type, on its device, "
-                          "and begin at a multiple of 16 bytes")
-    if page_table.dim() != 2 or page_table.shape[0] != B:
-        raise KernelError("page_table must have a row for every sequence")
-    i32 = torch.int32
-    if not (single and page_table.dtype is i32 and ctx_lens.dtype is i32 and page_table.is_contiguous()
-            and ctx_lens.is_contiguous() and page_table.get_device() == index and ctx_lens.get_device() == index):
-        for name, t, n in (("page_table", page_table, page_table.numel()), ("cu_seqlens", cu_seqlens, B + 1),
-                           ("ctx_lens", ctx_lens, B), ("seq_of_token", seq_of_token, T), ("positions", positions, T)):
-            if not _is(t, i32, n, index):
-                raise KernelError(f"{name} must be contiguous int32 of {n} elements on {q.device}")
-    if single and T != B:
-        raise KernelError("one token per sequence expected")
-    if max_ctx_len < 1 or max_new_tokens < 1:
-        raise KernelError("max_ctx_len and max_new_tokens must be at least 1")
-    return index
-
-
-_tickets = {}
-
-
-def _stream_tickets(n, like, index, stream) -> torch.Tensor:
-    """At least n tickets (int32, zero between launches) for a call on this stream."""
-    if torch.cuda.is_current_stream_capturing():
-        return like.new_zeros((n,), dtype=torch.int32)
-    tickets = _tickets.get((index, stream))
-    if tickets is None or tickets.numel() < n:
-        tickets = _tickets[index, stream] = like.new_zeros((max(n, 4096),), dtype=torch.int32)
-    return tickets
-
-
-def _decode_scratch(n_seqs, n_kv_heads, n_heads, head_dim, n_ctas, cluster, groups, q, index, stream):
-    """(part_o, part_ml, tickets) of a decode step's split work; zeros for none where no two CTAs share
-    a pair through memory.  The parts are this call's own.  The tickets, which are zero between
-    launches, are kept for each stream, whose calls run one after another; a captured call has its
-    own, zeroed in the graph, so that graphs may be replayed side by side."""
-    pairs = n_seqs * n_kv_heads
-    if cluster:
-        if groups == 1:
-            return None, 0, 0, 0
-        n_o, n_ml = pairs * groups * (n_heads // n_kv_heads) * head_dim, pairs * groups * 32
-    else:
-        slots = n_ctas + pairs
-        n_o, n_ml = slots * 16 * head_dim, slots * 16 * 2
-    part = q.new_empty((n_o + n_ml,), dtype=torch.float32)
-    tickets = _stream_tickets(pairs, q, index, stream)
-    return (part, tickets), part.data_ptr(), part.data_ptr() + 4 * n_o, tickets.data_ptr()
-
-
 @functools.lru_cache(maxsize=4096)
 def _bounded_decode_plan(n_seqs, n_kv_heads, n_heads, head_dim, blocks, splits, cluster, groups, n_sms):
     """(cluster, groups, n_ctas) of a decode step in which a query sees `blocks` pages."""
@@ -832,147 +752,26 @@ def _bounded_decode_plan(n_seqs, n_kv_heads, n_heads, head_dim, blocks, splits, 
     return cluster, groups, 0 if cluster else plan_decode_ctas(n_seqs, n_kv_heads, ctx, None, splits)
 
 
-@functools.lru_cache(maxsize=256)
-def _attention_kernels(n_heads, n_kv_heads, head_dim):
-    """(whether the mma.sync kernels take these sizes, whether the tcgen05 prefill does)"""
-    if n_kv_heads < 1:
-        raise KernelError("n_heads must be a multiple of n_kv_heads")
-    lib = library()
-    return (bool(lib.wpc_attention_mma_supports(n_heads, n_kv_heads, head_dim)),
-            bool(lib.wpc_attention_prefill_tc_supports(n_heads, n_kv_heads, head_dim)))
-
-
-def _attention_with_sinks(q, n_heads, n_kv_heads, head_dim, k_pages, v_pages, page_table, cu_seqlens, ctx_lens,
-                          seq_of_token, positions, scale, window, max_new_tokens, max_ctx_len, splits, mma_only,
-                          cluster, groups, sinks) -> torch.Tensor:
-    if window < 1:
-        raise KernelError(f"window must be positive, got {window}")
-    mma, tc = _attention_kernels(n_heads, n_kv_heads, head_dim)
-    T, B = q.shape[0], ctx_lens.numel()
-    fast = mma and q.dtype is torch.bfloat16 and q.stride(0) % 2 == 0 and q.data_ptr() % 4 == 0
-    single = fast and max_new_tokens == 1 and B <= 1024
-    index = _check_step(q, n_heads, n_kv_heads, head_dim, k_pages, v_pages, page_table, cu_seqlens, ctx_lens, seq_of_token,
-                        positions, max_new_tokens, max_ctx_len, single)
-    sinks, window = min(int(sinks), 1 << 30), min(int(window), 1 << 30)
-    if not fast:
-        return attention_plain(q, n_heads, n_kv_heads, head_dim, k_pages, v_pages, page_table, seq_of_token,
-                               positions, scale, window, max_ctx_len, sinks=sinks)
-    width = n_heads * head_dim
-    out = q.new_empty((T, width))
-    if not T:
-        return out
-    stream = _raw_stream(index)
-    shared = (q.data_ptr(), q.stride(0), out.data_ptr(), width, k_pages.data_ptr(), v_pages.data_ptr(),
-              page_table.data_ptr(), page_table.shape[1])
-    if single:
-        blocks = min(-(-max_ctx_len // PAGE), -(-window // PAGE) + 1 + -(-sinks // PAGE))
-        cluster, groups, n_ctas = _bounded_decode_plan(B, n_kv_heads, n_heads, head_dim, blocks, splits, cluster, groups,
-                                                       _sms_of.get(index) or sms())
-        own, part_o, part_ml, tickets = _decode_scratch(B, n_kv_heads, n_heads, head_dim, n_ctas, cluster, groups, q, index,
-                                                        stream)
-        _check("attention_decode_bounded", _typed_function("wpc_attention_decode_bounded")(
-            *shared, ctx_lens.data_ptr(), B, n_heads, n_kv_heads, head_dim, scale, window, sinks, n_ctas, cluster, groups,
-            part_o, part_ml, tickets, B * n_kv_heads, 0, 0, 0, 0, 0, 0, 0, 0, 0, stream))
-    elif not mma_only and tc and shared[1] % 8 == 0 and shared[0] % 16 == 0:
-        status = workspace(q.device)[2]
-        _check("attention_prefill_tc_bounded", _typed_function("wpc_attention_prefill_tc_bounded")(
-            *shared, cu_seqlens.data_ptr(), ctx_lens.data_ptr(), B, max_new_tokens, n_heads, n_kv_heads, head_dim, scale,
-            window, sinks, 0, status.data_ptr(), k_pages.shape[0], stream))
-    else:
-        _check("attention_prefill_bounded", _typed_function("wpc_attention_prefill_bounded")(
-            *shared, cu_seqlens.data_ptr(), ctx_lens.data_ptr(), B, max_new_tokens, n_heads, n_kv_heads, head_dim, scale,
-            window, sinks, 0, stream))
-    return out
-
-
-SUMS_KEYS = 256           # keys of a segment of csrc/attention_sums_tc.cu
-
-
-def _attention_with_sums(q, n_heads, n_kv_heads, head_dim, k_pages, v_pages, page_table, cu_seqlens, ctx_lens,
-                         seq_of_token, positions, scale, window, max_new_tokens, max_ctx_len, splits, mma_only,
-                         cluster, groups, sinks, weight_sums, stored_positions, token_positions) -> torch.Tensor:
+def _bounded_attention(q, n_heads, n_kv_heads, head_dim, k_pages, v_pages, page_table, cu_seqlens, ctx_lens, seq_of_token,
+                       positions, scale, window, max_new_tokens, max_ctx_len, splits, mma_only, cluster, groups, sinks,
+                       weight_sums, stored_positions, token_positions) -> torch.Tensor:
+    """Attention with a window and sinks, or with sums of weights: the plan of a single-token step is made
+    here, checks, memory and launches are csrc/host.cpp's."""
     global launch_count
-    if weight_sums is None or stored_positions is None or token_positions is None:
-        raise KernelError("weight_sums, stored_positions and token_positions come together")
-    if window or sinks:
-        raise KernelError("weights are summed over a cache that keeps everything: no window, no sinks")
-    mma, tc = _attention_kernels(n_heads, n_kv_heads, head_dim)
-    T, B, n_pages = q.shape[0], ctx_lens.numel(), k_pages.shape[0]
-    fast = mma and q.dtype is torch.bfloat16 and q.stride(0) % 2 == 0 and q.data_ptr() % 4 == 0
-    single = fast and max_new_tokens == 1 and B <= 1024
-    index = _check_step(q, n_heads, n_kv_heads, head_dim, k_pages, v_pages, page_table, cu_seqlens, ctx_lens, seq_of_token,
-                        positions, max_new_tokens, max_ctx_len, single)
-    shape = k_pages.shape[:3]
-    n = n_pages * n_kv_heads * PAGE
-    if weight_sums.shape != shape or not _is(weight_sums, torch.float32, n, index):
-        raise KernelError("weight_sums must be contiguous float32 [n_pages, n_kv_heads, PAGE]")
-    if stored_positions.shape != shape or not _is(stored_positions, torch.int32, n, index):
-        raise KernelError("stored_positions must be contiguous int32 [n_pages, n_kv_heads, PAGE]")
-    if not _is(token_positions, torch.int32, T, index):
-        raise KernelError("token_positions must be contiguous int32 [T]")
-    width = n_heads * head_dim
-    out = q.new_empty((T, width))
-    if not T:
-        return out
-    stream = _raw_stream(index)
-    status = workspace(q.device)[2].data_ptr()
-    q_ptr, k_ptr, table_ptr, table_width = q.data_ptr(), k_pages.data_ptr(), page_table.data_ptr(), page_table.shape[1]
-    shared = (q_ptr, q.stride(0), out.data_ptr(), width, k_ptr, v_pages.data_ptr(), table_ptr, table_width)
-    target = (n_pages, weight_sums.data_ptr(), stored_positions.data_ptr(), status, stream)
-    if single:
-        # a decode step: the scores stay in scratch memory until the rows' maxima and sums are known
+    if not q.is_cuda:
+        raise KernelError("q must be on a CUDA device")
+    n_ctas, n_sms = 0, _sms_of.get(q.get_device()) or sms()
+    if max_new_tokens == 1:
         blocks = -(-max_ctx_len // PAGE)
-        cluster, groups, n_ctas = _bounded_decode_plan(B, n_kv_heads, n_heads, head_dim, blocks, splits, cluster, groups,
-                                                       _sms_of.get(index) or sms())
-        own, part_o, part_ml, tickets = _decode_scratch(B, n_kv_heads, n_heads, head_dim, n_ctas, cluster, groups, q, index,
-                                                        stream)
-        scores = q.new_empty((B * n_heads * (blocks * PAGE + 2),), dtype=torch.float32)
-        _check("attention_decode_bounded", _typed_function("wpc_attention_decode_bounded")(
-            *shared, ctx_lens.data_ptr(), B, n_heads, n_kv_heads, head_dim, scale, 0, 0, n_ctas, cluster, groups,
-            part_o, part_ml, tickets, B * n_kv_heads, scores.data_ptr(), blocks * PAGE,
-            scores.data_ptr() + 4 * B * n_heads * blocks * PAGE, token_positions.data_ptr(), max_ctx_len, *target[:4], stream))
-        launch_count += 1                    # (the call launches two kernels)
-        return out
-    lse = q.new_empty((T, n_heads), dtype=torch.float32)
-    seqs = (cu_seqlens.data_ptr(), ctx_lens.data_ptr())
-    sizes = (B, n_heads, n_kv_heads, head_dim, scale)
-    on_tc = fast and tc and not mma_only and q.stride(0) % 8 == 0 and q_ptr % 16 == 0
-    if not fast:
-        attention_plain(q, n_heads, n_kv_heads, head_dim, k_pages, v_pages, page_table, seq_of_token, positions, scale,
-                        None, max_ctx_len, lse=lse, out=out)
-    elif on_tc:
-        _check("attention_prefill_tc_bounded", _typed_function("wpc_attention_prefill_tc_bounded")(
-            *shared, *seqs, B, max_new_tokens, n_heads, n_kv_heads, head_dim, scale, 0, 0, lse.data_ptr(), status, n_pages,
-            stream))
-        n_sms = _sms_of.get(index) or sms()
-        part = q.new_empty((2 * n_sms * SUMS_KEYS,), dtype=torch.float32)
-        tickets = _stream_tickets(B * n_kv_heads * -(-max_ctx_len // SUMS_KEYS), q, index, stream)
-        _check("weight_sums_tc", _typed_function("wpc_weight_sums_tc")(
-            q_ptr, q.stride(0), T, k_ptr, table_ptr, table_width, *seqs, token_positions.data_ptr(), lse.data_ptr(), *sizes,
-            max_new_tokens, max_ctx_len, *target[:4], part.data_ptr(), tickets.data_ptr(), tickets.numel(), stream))
-        return out
-    else:
-        _check("attention_prefill_bounded", _typed_function("wpc_attention_prefill_bounded")(
-            *shared, *seqs, B, max_new_tokens, n_heads, n_kv_heads, head_dim, scale, 0, 0, lse.data_ptr(), stream))
-    _check("weight_sums_plain", _typed_function("wpc_weight_sums_plain")(
-        q_ptr, q.stride(0), _code(q.dtype), k_ptr, table_ptr, table_width, *seqs, token_positions.data_ptr(), lse.data_ptr(),
-        *sizes, max_ctx_len, *target))
+        if window:
+            blocks = min(blocks, -(-window // PAGE) + 1 + -(-sinks // PAGE))
+        cluster, groups, n_ctas = _bounded_decode_plan(ctx_lens.numel(), n_kv_heads, n_heads, head_dim, blocks, splits, cluster,
+                                                       groups, n_sms)
+    out = host().attention(q, n_heads, n_kv_heads, head_dim, k_pages, v_pages, page_table, cu_seqlens, ctx_lens, seq_of_token,
+                           positions, scale, window or 0, max_new_tokens, max_ctx_len, mma_only, sinks, weight_sums,
+                           stored_positions, token_positions, cluster or 0, groups, n_ctas, n_sms, workspace(q.device)[2])
+    launch_count += 1 if weight_sums is None else 2
     return out
-
-
-def _record(weight_sums, stored_positions, page_table):
-    """Checks the two records of one layer or of several and a page table; returns
-    (device index, layers, pages, KV heads, sequences)."""
-    index = _on_current_device(weight_sums, "weight_sums")
-    shape = weight_sums.shape
-    n = weight_sums.numel()
-    if not (len(shape) in (3, 4) and shape[-1] == PAGE and _is(weight_sums, torch.float32, n, index)):
-        raise KernelError("weight_sums must be contiguous float32 [layers, n_pages, n_kv_heads, PAGE] (or of one layer)")
-    if stored_positions.shape != shape or not _is(stored_positions, torch.int32, n, index):
-        raise KernelError("stored_positions must be contiguous int32 of weight_sums' shape")
-    if page_table.dim() != 2 or not _is(page_table, torch.int32, page_table.numel(), index):
-        raise KernelError("page_table must be contiguous int32 [B, width]")
-    return index, 1 if len(shape) == 3 else shape[0], shape[-3], shape[-2], page_table.shape[0]
 
 
 def select_kept(weight_sums: torch.Tensor, stored_positions: torch.Tensor, page_table: torch.Tensor,
@@ -991,16 +790,12 @@ def select_kept(weight_sums: torch.Tensor, stored_positions: torch.Tensor, page_
     if not (keep >= 1 and sinks >= 0 and recent >= 0 and sinks + recent <= keep):
         raise KernelError(f"keep must be at least 1 and hold the sinks and the recent positions, got keep {keep}, "
                           f"sinks {sinks}, recent {recent}")
-    index, layers, n_pages, n_kv, B = _record(weight_sums, stored_positions, page_table)
-    for name, t in (("stored_lens", stored_lens), ("next_positions", next_positions)):
-        if not _is(t, torch.int32, B, index):
-            raise KernelError(f"{name} must be contiguous int32 [B]")
-    kept = weight_sums.new_empty((B, n_kv, keep) if weight_sums.dim() == 3 else (layers, B, n_kv, keep), dtype=torch.int32)
-    if kept.numel():
-        _check("select_kept", _typed_function("wpc_select_kept")(
-            weight_sums.data_ptr(), stored_positions.data_ptr(), page_table.data_ptr(), page_table.shape[1],
-            stored_lens.data_ptr(), next_positions.data_ptr(), layers, B, n_kv, n_pages, keep, sinks, recent,
-            kept.data_ptr(), workspace(weight_sums.device)[2].data_ptr(), _raw_stream(index)))
+    global launch_count
+    if not weight_sums.is_cuda:
+        raise KernelError("weight_sums must be on a CUDA device")
+    kept = host().select_kept(weight_sums, stored_positions, page_table, stored_lens, next_positions, keep, sinks, recent,
+                              workspace(weight_sums.device)[2])
+    launch_count += 1
     return kept
 
 
@@ -1011,19 +806,11 @@ def move_kept_(k_pages: torch.Tensor, v_pages: torch.Tensor, weight_sums: torch.
     kept[.., i] is i, -1 (nothing), or at least `keep`, kept's last size: an entry that is named
     otherwise, or that has no page, stays where it is, and the device error word says 1001.
     Afterwards the first `keep` places hold what was kept, and the pages behind them may go."""
-    index, layers, n_pages, n_kv, B = _record(weight_sums, stored_positions, page_table)
-    shape = weight_sums.shape
-    for name, t in (("k_pages", k_pages), ("v_pages", v_pages)):
-        if t.shape[:-1] != shape or t.dtype not in (torch.float32, torch.bfloat16) or not _is(t, t.dtype, t.numel(), index):
-            raise KernelError(f"{name} must be contiguous [.., n_pages, n_kv_heads, PAGE, head_dim] like weight_sums")
-    if kept.dim() != len(shape) or kept.shape[:-1] != shape[:-3] + (B, n_kv) or not _is(kept, torch.int32, kept.numel(), index):
-        raise KernelError("kept must be contiguous int32 [.., B, n_kv_heads, keep]")
-    if kept.numel():
-        _check("move_kept", _typed_function("wpc_move_kept")(
-            k_pages.data_ptr(), v_pages.data_ptr(), k_pages.shape[-1] * k_pages.element_size(),
-            v_pages.shape[-1] * v_pages.element_size(), weight_sums.data_ptr(), stored_positions.data_ptr(),
-            page_table.data_ptr(), page_table.shape[1], kept.data_ptr(), layers, B, n_kv, n_pages, kept.shape[-1],
-            workspace(weight_sums.device)[2].data_ptr(), _raw_stream(index)))
+    global launch_count
+    if not weight_sums.is_cuda:
+        raise KernelError("weight_sums must be on a CUDA device")
+    host().move_kept(k_pages, v_pages, weight_sums, stored_positions, page_table, kept, workspace(weight_sums.device)[2])
+    launch_count += 1
 
 
 def plan_decode_ctas(n_seqs: int, n_kv_heads: int, max_ctx_len: int, window: Optional[int],
