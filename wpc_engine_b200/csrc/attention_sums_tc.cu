@@ -252,16 +252,7 @@ prefill_sums_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     *(uint4*)(base + 2 * W::K_BYTES + half * W::Q_HALF + rows * 128 + in * 16) = make_uint4(0, 0, 0, 0);
   }
   fence_async_smem();
-  pdl_wait();
-  // (tensor memory only now: the kernel ahead may still need it)
-  if (warp == ST_MMA_WARP) tmem_alloc(&tmem_holder, 512);
-  fence_before_sync();
-  __syncthreads();
-  fence_after_sync();
-  const uint32_t tmem = tmem_holder;
-  // (only now: the kernel behind may hold tensor memory while it waits for this one, so every CTA
-  // of this one must have got its own first)
-  if (!late_trigger) pdl_trigger();
+  __syncthreads();                                           // s_found is there, and the barriers and zeros are
   Segment sg;
   sg.b = s_found[0] / work.key_tiles;
   sg.kt = s_found[0] % work.key_tiles;
@@ -273,42 +264,68 @@ prefill_sums_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
   sg.n = min(sg.all - sg.t0, sg.left);
   sg.load(work);
 
+  const bool copies = warp == ST_COPY_WARP && lane == 0 && !starve;
+  // the copies of a segment's keys, and of its j-th query tile (number i since the kernel's start)
+  auto copy_keys = [&](int s) {
+    const int* table = t.page_table + (size_t)sg.b * t.table_width;
+    int page[ST_KEYS / WPC_PAGE];                            // (all look-ups on their way before the first is needed)
+#pragma unroll
+    for (int p = 0; p < ST_KEYS / WPC_PAGE; ++p) {
+      const int block = sg.kt * (ST_KEYS / WPC_PAGE) + p;
+      page[p] = block * WPC_PAGE < sg.L && block < t.table_width ? table[block] : 0;
+    }
+    pdl_wait();                                              // (at once after the first time)
+    mbar_expect_tx(k_full + (s & 1), W::K_BYTES);
+#pragma unroll
+    for (int p = 0; p < ST_KEYS / WPC_PAGE; ++p) {
+      const int row = (min(max(page[p], 0), t.n_pages - 1) * work.nkv + sg.g) * WPC_PAGE;
+#pragma unroll
+      for (int hb = 0; hb < W::NB; ++hb)
+        tma_load_2d(k_s + (s & 1) * W::K_BYTES + hb * W::K_HALF + p * (WPC_PAGE * 128), &map_k, hb * 64, row, k_full + (s & 1));
+    }
+  };
+  auto copy_queries = [&](int i, int j) {
+    const int st = i % NS;
+    mbar_expect_tx(q_full + st, rows * 128 * W::NB);
+#pragma unroll
+    for (int hb = 0; hb < W::NB; ++hb)
+      tma_load_3d(q_s + st * W::Q_BYTES + hb * W::Q_HALF, &map_q, hb * 64, sg.g * work.n_rep, sg.tok0 + sg.token(work, j), q_full + st);
+  };
+  // the first copies start with the dependency wait's end, beside the allocation of tensor memory
+  const int primed = min(NS, sg.n);
+  if (copies) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&map_k) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&map_q) : "memory");
+    copy_keys(0);
+    for (int j = 0; j < primed; ++j) copy_queries(j, j);
+  }
+  __syncwarp();
+  pdl_wait();
+  // (tensor memory only now: the kernel ahead may still need it)
+  if (warp == ST_MMA_WARP) tmem_alloc(&tmem_holder, 512);
+  fence_before_sync();
+  __syncthreads();
+  fence_after_sync();
+  const uint32_t tmem = tmem_holder;
+  // (only now: the kernel behind may hold tensor memory while it waits for this one, so every CTA
+  // of this one must have got its own first)
+  if (!late_trigger) pdl_trigger();
   if (warp == ST_COPY_WARP) {
-    if (lane == 0 && !starve) {
-      asm volatile("prefetch.tensormap [%0];" ::"l"(&map_k) : "memory");
-      asm volatile("prefetch.tensormap [%0];" ::"l"(&map_q) : "memory");
-      int s = 0, i = 0;                                      // segments and query tiles so far
+    if (copies) {
+      int s = 0, i = primed;                                 // segments and query tiles so far
       bool ok = true;
-      do {
-        const int* table = t.page_table + (size_t)sg.b * t.table_width;
-        ok = mbar_wait(k_empty + (s & 1), ((s >> 1) & 1) ^ 1, wait_ns);
-        if (!ok) break;
-        mbar_expect_tx(k_full + (s & 1), W::K_BYTES);
-        int page[ST_KEYS / WPC_PAGE];                        // (all look-ups on their way before the first is needed)
-#pragma unroll
-        for (int p = 0; p < ST_KEYS / WPC_PAGE; ++p) {
-          const int block = sg.kt * (ST_KEYS / WPC_PAGE) + p;
-          page[p] = block * WPC_PAGE < sg.L && block < t.table_width ? table[block] : 0;
-        }
-#pragma unroll
-        for (int p = 0; p < ST_KEYS / WPC_PAGE; ++p) {
-          const int row = (min(max(page[p], 0), t.n_pages - 1) * work.nkv + sg.g) * WPC_PAGE;
-#pragma unroll
-          for (int hb = 0; hb < W::NB; ++hb)
-            tma_load_2d(k_s + (s & 1) * W::K_BYTES + hb * W::K_HALF + p * (WPC_PAGE * 128), &map_k, hb * 64, row, k_full + (s & 1));
-        }
-        for (int j = 0; j < sg.n; ++j, ++i) {
-          const int st = i % NS;
-          ok = mbar_wait(q_empty + st, ((i / NS) & 1) ^ 1, wait_ns);
+      for (;;) {
+        for (int j = s == 0 ? primed : 0; j < sg.n; ++j, ++i) {
+          ok = mbar_wait(q_empty + i % NS, ((i / NS) & 1) ^ 1, wait_ns);
           if (!ok) break;
-          mbar_expect_tx(q_full + st, rows * 128 * W::NB);
-#pragma unroll
-          for (int hb = 0; hb < W::NB; ++hb)
-            tma_load_3d(q_s + st * W::Q_BYTES + hb * W::Q_HALF, &map_q, hb * 64, sg.g * work.n_rep,
-                        sg.tok0 + sg.token(work, j), q_full + st);
+          copy_queries(i, j);
         }
         ++s;
-      } while (ok && sg.next(work));
+        if (!ok || !sg.next(work)) break;
+        ok = mbar_wait(k_empty + (s & 1), ((s >> 1) & 1) ^ 1, wait_ns);
+        if (!ok) break;
+        copy_keys(s);
+      }
       if (!ok) atomicExch(&failed, 1);
     }
     if (late_trigger) pdl_trigger();
