@@ -129,7 +129,7 @@ int wpc_weight_sums_decode(const float* scores, int score_stride, const float* r
                            cudaStream_t stream);
 int wpc_weight_sums_plain(const void* q, int q_stride, int dtype, const void* k_pages, const int* page_table,
                           int table_width, const int* cu_seqlens, const int* ctx_lens, const int* token_positions,
-                          const float* lse, int B, int nh, int nkv, int hd, float scale, int max_ctx, int n_pages,
+                          const float* lse, int B, int nh, int nkv, int hd, float scale, int max_new, int max_ctx, int n_pages,
                           float* weight_sums, int* stored_positions, int* status, cudaStream_t stream);
 
 // the same as wpc_weight_sums_plain on the tensor cores (attention_sums_tc.cu): bfloat16, head sizes 64 and 128
@@ -138,6 +138,12 @@ int wpc_weight_sums_tc(const void* q, int q_stride, int n_tokens, const void* k_
                        const float* lse, int B, int nh, int nkv, int hd, float scale, int max_new, int max_ctx,
                        int n_pages, float* weight_sums, int* stored_positions, int* status, float* part, int* tickets,
                        int n_tickets, cudaStream_t stream);
+
+// the same with mma.sync (attention_sums_mma.cu): bfloat16, head sizes that are multiples of 16 up to 128
+int wpc_weight_sums_mma(const void* q, int q_stride, const void* k_pages, const int* page_table, int table_width,
+                        const int* cu_seqlens, const int* ctx_lens, const int* token_positions, const float* lse,
+                        int B, int nh, int nkv, int hd, float scale, int max_new, int max_ctx, int n_pages,
+                        float* weight_sums, int* stored_positions, int* status, cudaStream_t stream);
 
 // eviction.cu.  kept: int32 [layers][B][nkv][keep], the entry that belongs at each place of the kept
 // part (-1 behind a shorter sequence).  weight_sums, stored_positions: [layers][n_pages][nkv][64].

@@ -214,10 +214,17 @@ at::Tensor attention(const Args& a) {
     lse = empty({T, nh}, at::kFloat, device);
     lse_p = lse.data_ptr<float>();
   }
-  const bool on_tc = fast && !mma_only && q_stride % 8 == 0 && address(q) % 16 == 0 && wpc_attention_prefill_tc_supports(nh, nkv, hd);
+  const bool aligned = fast && q_stride % 8 == 0 && address(q) % 16 == 0;      // q rows can be copied 16 bytes at a time
+  const bool on_tc = aligned && !mma_only && wpc_attention_prefill_tc_supports(nh, nkv, hd);
   if (!fast) {
     const int keys = window ? (int)std::min<long>(max_ctx, (long)window + sinks) : max_ctx;
-    const int splits = (int)std::max<long>(1, std::min<long>(keys / 256, 2L * n_sms / std::max<long>((long)T * nh, 1)));
+    // Blocks that share a query's keys: about 64 keys each, at most 16, and no more blocks than eight to an SM.
+    // Four sequences of up to 1,000 positions, window 257, 14 heads of 64: 1 block 15.4 us, 4 (the rule) 9.5,
+    // 12 11.2; one sequence, window 2,048: 1 block 92.5, 16 (the rule) 16.5, 32 18.2.
+    const long rows = std::max<long>((long)T * nh, 1);
+    // Without a window the split is that of the ordinary attention, so that keeping sums changes no bit of it.
+    const int splits = (int)std::max<long>(1, window ? std::min<long>(std::min(keys / 64, 16), 8L * n_sms / rows)
+                                                     : std::min<long>(keys / 256, 2L * n_sms / rows));
     at::Tensor part;
     if (splits > 1) part = empty({(long)T * nh * splits * (hd + 2)}, at::kFloat, device);
     launched("attention_plain", wpc_attention_plain_bounded(
@@ -242,10 +249,14 @@ at::Tensor attention(const Args& a) {
         q.data_ptr(), q_stride, T, k.data_ptr(), table_p, width, cu_p, ctx_p, told, lse_p, B, nh, nkv, hd, scale, max_new,
         max_ctx, n_pages, weight_sums, stored, status, part.data_ptr<float>(), tickets.data_ptr<int>(), (int)tickets.numel(),
         stream));
+  } else if (aligned) {
+    launched("weight_sums_mma", wpc_weight_sums_mma(
+        q.data_ptr(), q_stride, k.data_ptr(), table_p, width, cu_p, ctx_p, told, lse_p, B, nh, nkv, hd, scale, max_new, max_ctx,
+        n_pages, weight_sums, stored, status, stream));
   } else {
     launched("weight_sums_plain", wpc_weight_sums_plain(
         q.data_ptr(), q_stride, type == at::kFloat ? 0 : 1, k.data_ptr(), table_p, width, cu_p, ctx_p, told, lse_p, B, nh, nkv,
-        hd, scale, max_ctx, n_pages, weight_sums, stored, status, stream));
+        hd, scale, max_new, max_ctx, n_pages, weight_sums, stored, status, stream));
   }
   return out;
 }
