@@ -176,6 +176,24 @@ def test_infinite_and_nan_values_in_masked_places_do_not_matter():
                     assert all(torch.equal(x, y) for x, y in zip(attend(how), was)), (n_new, dtype, sums, how)
 
 
+@pytest.mark.parametrize("how", [dict(cluster=0), dict(splits=2), dict(cluster=2), dict(cluster=3, groups=2)])
+@pytest.mark.parametrize("sums", [False, True])
+def test_a_sequence_without_positions_gives_zeros(how, sums):
+    s = Step(torch.bfloat16, 14, 2, 64, [300, 64, 90], [1, 1, 1], None if sums else 100, 0 if sums else 5, seed=1)
+    whole = s.want()
+    s.ctx = ints([300, 0, 90])
+    record = s.record()
+    torch.full((1 << 22,), math.nan, device=DEV)             # (what the allocator hands out next)
+    if sums:
+        got = s.attend(weight_sums=record[0], stored_positions=record[1], token_positions=s.pos, **how)
+        assert torch.equal(record[0][int(s.table[1, 0])], s.record()[0][int(s.table[1, 0])])
+    else:
+        got = s.attend(sinks=5, **how)
+    assert bool((got[1] == 0).all())
+    off = (got.double().cpu() - whole[0]).abs()[[0, 2]]
+    assert bool((off <= plain.out_bound(whole[0], whole[1], whole[2], torch.bfloat16, 300)[[0, 2]]).all())
+
+
 def test_sinks_without_a_window_change_nothing():
     s = Step(torch.bfloat16, 14, 2, 64, [300, 70], [40, 1], seed=1)
     assert torch.equal(s.attend(sinks=4), s.attend())
@@ -526,6 +544,10 @@ def test_refusals():
     refused("stored_positions must be", s.attend, **dict(ok, stored_positions=stored.long()))
     refused("token_positions must be", s.attend, **dict(ok, token_positions=s.pos.repeat(2)))
     refused("token_positions must be", s.attend, **dict(ok, token_positions=s.pos.cpu()))
+    s.max_ctx, w.max_ctx = 6 * PAGE + 1, 6 * PAGE + 1
+    refused("an entry for every block", s.attend, **ok)
+    refused("an entry for every block", w.attend, sinks=4)
+    s.max_ctx = w.max_ctx = 300
     full = w.table
     w.table = full[:1]
     refused("a row for every sequence", w.attend, sinks=4)

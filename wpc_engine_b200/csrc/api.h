@@ -68,7 +68,7 @@ int wpc_attention_plain(const void* q, int q_stride, void* out, int out_stride, 
 int wpc_attention_plain_bounded(const void* q, int q_stride, void* out, int out_stride, int dtype,
                                 const void* k_pages, const void* v_pages, const int* page_table, int table_width,
                                 const int* seq_of_token, const int* positions, int T, int nh, int nkv, int hd,
-                                float scale, int window, int sinks, int n_splits, float* part, float* lse,
+                                float scale, int window, int sinks, int n_splits, float* part, float* lse, int n_pages,
                                 cudaStream_t stream);
 
 int wpc_attention_mma_supports(int nh, int nkv, int hd);
@@ -117,7 +117,7 @@ int wpc_attention_decode_bounded(const void* q, int q_stride, void* out, int out
 int wpc_attention_prefill_bounded(const void* q, int q_stride, void* out, int out_stride, const void* k_pages,
                                   const void* v_pages, const int* page_table, int table_width, const int* cu_seqlens,
                                   const int* ctx_lens, int B, int max_new, int nh, int nkv, int hd, float scale,
-                                  int window, int sinks, float* lse, cudaStream_t stream);
+                                  int window, int sinks, float* lse, int n_pages, cudaStream_t stream);
 
 // attention_sums.cu: the weight that each cached entry received, added to weight_sums
 // [n_pages][nkv][64] (an entry of the step's own tokens begins with it, and its place in

@@ -15,13 +15,14 @@ static int decode_bounded(const void* q, int q_stride, void* out, int out_stride
                           const void* v_pages, const int* page_table, int table_width, const int* ctx_lens,
                           int B, int nh, int nkv, int hd, float scale, int window, int sinks, int n_ctas,
                           int cluster, int groups, float* part_o, float* part_ml, int* counters, int n_counters,
-                          float* scores, int score_stride, float* row_ml, cudaStream_t stream) {
+                          float* scores, int score_stride, float* row_ml, int n_pages, cudaStream_t stream) {
   if (B <= 0) return 0;
   if (!wpc_attention_mma_supports(nh, nkv, hd) || (q_stride % 2) || (out_stride % 2)) return WPC_ERR_UNSUPPORTED;
+  if (n_pages < 1) return WPC_ERR_BAD_ARGUMENT;
   const bool sums = scores != nullptr;
   if (sums ? (!row_ml || score_stride < 64 || score_stride % 64 || window > 0 || sinks != 0) : (sinks < 1 || window < 1))
     return WPC_ERR_BAD_ARGUMENT;
-  const fa::Extra x{sinks, score_stride, scores, (float2*)row_ml, nullptr};
+  const fa::Extra x{sinks, score_stride, scores, (float2*)row_ml, nullptr, n_pages};
   if (cluster) {
     if ((nh / nkv) * hd > fa::CLUSTER_DECODE_MAX_OUT) return WPC_ERR_UNSUPPORTED;
     if (cluster < 2 || cluster > fa::CLUSTER_DECODE_MAX_RANKS || groups < 1 ||
@@ -61,7 +62,7 @@ int wpc_attention_decode_bounded(const void* q, int q_stride, void* out, int out
                                  cudaStream_t stream) {
   const int rc = decode_bounded(q, q_stride, out, out_stride, k_pages, v_pages, page_table, table_width, ctx_lens, B, nh,
                                 nkv, hd, scale, window, sinks, n_ctas, cluster, groups, part_o, part_ml, counters,
-                                n_counters, scores, score_stride, row_ml, stream);
+                                n_counters, scores, score_stride, row_ml, n_pages, stream);
   if (rc || !scores) return rc;
   return wpc_weight_sums_decode(scores, score_stride, row_ml, page_table, table_width, ctx_lens, token_positions, B, nh,
                                 nkv, max_ctx, n_pages, weight_sums, stored_positions, status, stream);
@@ -70,11 +71,12 @@ int wpc_attention_decode_bounded(const void* q, int q_stride, void* out, int out
 int wpc_attention_prefill_bounded(const void* q, int q_stride, void* out, int out_stride, const void* k_pages,
                                   const void* v_pages, const int* page_table, int table_width, const int* cu_seqlens,
                                   const int* ctx_lens, int B, int max_new, int nh, int nkv, int hd, float scale,
-                                  int window, int sinks, float* lse, cudaStream_t stream) {
+                                  int window, int sinks, float* lse, int n_pages, cudaStream_t stream) {
   if (B <= 0 || max_new <= 0) return 0;
+  if (n_pages < 1) return WPC_ERR_BAD_ARGUMENT;
   if (!wpc_attention_mma_supports(nh, nkv, hd) || (q_stride % 2) || (out_stride % 2)) return WPC_ERR_UNSUPPORTED;
   if (lse ? (window > 0 || sinks != 0) : (sinks < 1 || window < 1)) return WPC_ERR_BAD_ARGUMENT;
-  const fa::Extra x{sinks, 0, nullptr, nullptr, lse};
+  const fa::Extra x{sinks, 0, nullptr, nullptr, lse, n_pages};
   if (lse) {
     WPC_DISPATCH_HD(hd, fa::launch_prefill<HD, fa::MODE_SUMS>(q, q_stride, out, out_stride, k_pages, v_pages, page_table,
                                                              table_width, cu_seqlens, ctx_lens, B, max_new, nh, nkv,

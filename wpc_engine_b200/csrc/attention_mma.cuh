@@ -90,12 +90,17 @@ struct Extra {
   float* scores;         // MODE_SUMS, decode: [B * nkv][heads of a group][score_stride], log2 domain
   float2* row_ml;        // MODE_SUMS, decode: [B][nh] (maximum, 1 / sum), log2 domain
   float* lse;            // MODE_SUMS, prefill: [T][nh] maximum + log2(sum)
+  int n_pages;           // pages of the cache: a page number outside them is read as the nearest one
 };
 
 // Pages of the sinks that lie wholly before block `first`.
 template <int MODE>
 __device__ __forceinline__ int sink_blocks(const Extra& x, int first) {
   return MODE == MODE_SINKS ? min((x.sinks + WPC_PAGE - 1) / WPC_PAGE, first) : 0;
+}
+template <int MODE>
+__device__ __forceinline__ int cache_page(const Extra& x, int page) {
+  return MODE == MODE_PLAIN ? page : min(page, x.n_pages - 1);     // (negative ones are the loads' own care)
 }
 // The block that number `blk` of a query's range stands for (see the head of this file).
 template <int MODE>
@@ -319,6 +324,16 @@ decode_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, __nv_bfloat16* 
     }
   }
   __syncthreads();
+  if (MODE != MODE_PLAIN && blockIdx.x == gridDim.x - 1) {
+    // a sequence of no positions has no units: its rows are zeros
+    bool waited = false;
+    for (int e = 0; e < B; ++e)
+      if (s_cum[e + 1] == s_cum[e]) {
+        if (!waited) pdl_wait();
+        waited = true;
+        for (int i = tid; i < nh * HD; i += THREADS) out[(size_t)e * out_stride + i] = __float2bfloat16_rn(0.f);
+      }
+  }
   const int U = s_cum[B];
   const int per = (U + (int)gridDim.x - 1) / (int)gridDim.x;
   const int u0 = blockIdx.x * per, u1 = min(U, u0 + per);
@@ -356,11 +371,11 @@ decode_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, __nv_bfloat16* 
     // would put a trip to L2 before every copy
     const int* gtable = page_table + (size_t)b * table_width;
     const int n_seg = blk1 - blk0;
-    for (int i = tid; i < min(n_seg, MAX_SEGMENT_PAGES); i += THREADS) s_pages[i] = gtable[real_block<MODE>(blk0 + i, first, ns)];
+    for (int i = tid; i < min(n_seg, MAX_SEGMENT_PAGES); i += THREADS) s_pages[i] = cache_page<MODE>(x, gtable[real_block<MODE>(blk0 + i, first, ns)]);
     __syncthreads();                                     // the page numbers are in shared memory for every thread
     auto page_of = [&](int blk) {
       const int i = blk - blk0;
-      return i < MAX_SEGMENT_PAGES ? s_pages[i] : gtable[real_block<MODE>(blk, first, ns)];
+      return i < MAX_SEGMENT_PAGES ? s_pages[i] : cache_page<MODE>(x, gtable[real_block<MODE>(blk, first, ns)]);
     };
 
     // A ring of DECODE_STAGES pages: two are in flight while one is computed.  Up to here only
@@ -622,11 +637,11 @@ decode_cluster_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, __nv_bf
   const int blk0 = g_blk0 + rank * base + min(rank, extra), blk1 = blk0 + base + (rank < extra ? 1 : 0);
   const int* gtable = page_table + (size_t)b * table_width;
   const int n_seg = blk1 - blk0;
-  for (int i = tid; i < min(n_seg, CLUSTER_SEGMENT_PAGES); i += THREADS) s_pages[i] = gtable[real_block<MODE>(blk0 + i, first, ns)];
+  for (int i = tid; i < min(n_seg, CLUSTER_SEGMENT_PAGES); i += THREADS) s_pages[i] = cache_page<MODE>(x, gtable[real_block<MODE>(blk0 + i, first, ns)]);
   __syncthreads();                                       // the page numbers are in shared memory for every thread
   auto page_of = [&](int blk) {
     const int i = blk - blk0;
-    return i < CLUSTER_SEGMENT_PAGES ? s_pages[i] : gtable[real_block<MODE>(blk, first, ns)];
+    return i < CLUSTER_SEGMENT_PAGES ? s_pages[i] : cache_page<MODE>(x, gtable[real_block<MODE>(blk, first, ns)]);
   };
 
   // The first pages of the ring are started ahead of the dependency wait, except the sequence's
@@ -869,7 +884,7 @@ prefill_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, __nv_bfloat16*
   const int tile_lo = (window > 0 && tile_pos_lo - window + 1 > 0) ? tile_pos_lo - window + 1 : 0;
   const int first = tile_lo / PAGE, ns = sink_blocks<MODE>(x, first);
   const int blk0 = first - ns, blk1 = tile_pos_hi / PAGE + 1;
-  auto page_of = [&](int blk) { return table[real_block<MODE>(blk, first, ns)]; };
+  auto page_of = [&](int blk) { return cache_page<MODE>(x, table[real_block<MODE>(blk, first, ns)]); };
   const int lo_lo = (window > 0 && p_lo - window + 1 > 0) ? p_lo - window + 1 : 0;
   const int lo_hi = (window > 0 && p_hi - window + 1 > 0) ? p_hi - window + 1 : 0;
   // this warp's rows see keys in [warp_lo, warp_hi]

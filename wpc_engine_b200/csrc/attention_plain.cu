@@ -31,7 +31,7 @@ attention_plain_kernel(const T* __restrict__ q, int q_stride, T* __restrict__ ou
                        const int* __restrict__ page_table, int table_width,
                        const int* __restrict__ seq_of_token, const int* __restrict__ positions,
                        int nh, int nkv, int hd, float scale, int window, int sinks, float* __restrict__ lse,
-                       float* __restrict__ part) {
+                       int n_pages, float* __restrict__ part) {
   pdl_trigger();
   pdl_wait();
   q = after_wait(q);
@@ -67,7 +67,7 @@ attention_plain_kernel(const T* __restrict__ q, int q_stride, T* __restrict__ ou
     float m_loc = -INFINITY;
     for (int j = threadIdx.x; j < cn; j += AP_THREADS) {
       const int p = lo + c0 + j + (lo + c0 + j < ns ? 0 : skipped);
-      const int page = max(table[p / WPC_PAGE], 0);
+      const int page = min(max(table[p / WPC_PAGE], 0), n_pages - 1);
       const T* kr = k_pages + (((size_t)page * nkv + kvh) * WPC_PAGE + p % WPC_PAGE) * hd;
       float dot = 0.f;
       if ((hd & 3) == 0) {                              // the same order of additions, four elements a load
@@ -106,7 +106,7 @@ attention_plain_kernel(const T* __restrict__ q, int q_stride, T* __restrict__ ou
           const int at = lo + c0 + j, p = at + (at < ns ? 0 : skipped);
           const int in_page = p % WPC_PAGE;
           const int n = min(at < ns ? min(cn - j, ns - at) : cn - j, WPC_PAGE - in_page);
-          const T* vr = v_pages + (((size_t)max(table[p / WPC_PAGE], 0) * nkv + kvh) * WPC_PAGE + in_page) * hd + d;
+          const T* vr = v_pages + (((size_t)min(max(table[p / WPC_PAGE], 0), n_pages - 1) * nkv + kvh) * WPC_PAGE + in_page) * hd + d;
           for (int i = 0; i < n; ++i) a = fmaf(ps[j + i], to_float(vr[(size_t)i * hd]), a);
           j += n;
         }
@@ -180,25 +180,25 @@ extern "C" int wpc_attention_plain(const void* q, int q_stride, void* out, int o
                                    cudaStream_t stream) {
   return wpc_attention_plain_bounded(q, q_stride, out, out_stride, dtype, k_pages, v_pages, page_table, table_width,
                                      seq_of_token, positions, T, nh, nkv, hd, scale, window, 0, n_splits, part, nullptr,
-                                     stream);
+                                     0x7fffffff, stream);
 }
 
 extern "C" int wpc_attention_plain_bounded(const void* q, int q_stride, void* out, int out_stride, int dtype,
                                            const void* k_pages, const void* v_pages, const int* page_table,
                                            int table_width, const int* seq_of_token, const int* positions, int T,
                                            int nh, int nkv, int hd, float scale, int window, int sinks, int n_splits,
-                                           float* part, float* lse, cudaStream_t stream) {
+                                           float* part, float* lse, int n_pages, cudaStream_t stream) {
   // n_splits > 1: that many blocks share the keys of each query; part: float32 scratch of
   // T * nh * n_splits * (hd + 2) elements for their partial results
   if (T <= 0) return 0;
   if (hd < 1 || hd > 2 * AP_THREADS || nkv < 1 || nh % nkv) return WPC_ERR_UNSUPPORTED;
-  if (n_splits < 1 || n_splits > 65535 || (n_splits > 1 && !part) || sinks < 0) return WPC_ERR_BAD_ARGUMENT;
+  if (n_splits < 1 || n_splits > 65535 || (n_splits > 1 && !part) || sinks < 0 || n_pages < 1) return WPC_ERR_BAD_ARGUMENT;
   const size_t smem = (size_t)(hd + AP_CHUNK) * sizeof(float);
   dim3 grid(T, nh, n_splits);
   WPC_DISPATCH_DTYPE(dtype, Tt,
                      wpc::launch(attention_plain_kernel<Tt>, grid, AP_THREADS, smem, stream, 
                          (const Tt*)q, q_stride, (Tt*)out, out_stride, (const Tt*)k_pages, (const Tt*)v_pages,
-                         page_table, table_width, seq_of_token, positions, nh, nkv, hd, scale, window, sinks, lse, part));
+                         page_table, table_width, seq_of_token, positions, nh, nkv, hd, scale, window, sinks, lse, n_pages, part));
   int rc = launch_status();
   if (rc || n_splits == 1) return rc;
   WPC_DISPATCH_DTYPE(dtype, Tt,

@@ -154,6 +154,7 @@ at::Tensor attention(const Args& a) {
   need_ints(pos, "positions", T, device);
   if (max_new < 1 || max_ctx < 1) refuse("max_ctx_len and max_new_tokens must be at least 1");
   const int width = as_int(table.size(1), "page_table's width");
+  if ((max_ctx + PAGE - 1) / PAGE > width || n_pages < 1) refuse("page_table must have an entry for every block of max_ctx_len positions");
   float* weight_sums = nullptr;
   int *stored = nullptr, *told = nullptr;
   if (sums) {
@@ -230,7 +231,7 @@ at::Tensor attention(const Args& a) {
     launched("attention_plain", wpc_attention_plain_bounded(
         q.data_ptr(), q_stride, out.data_ptr(), out_stride, type == at::kFloat ? 0 : 1, k.data_ptr(), v.data_ptr(), table_p,
         width, seq.data_ptr<int>(), pos.data_ptr<int>(), T, nh, nkv, hd, scale, window, sinks, splits,
-        splits > 1 ? part.data_ptr<float>() : nullptr, lse_p, stream));
+        splits > 1 ? part.data_ptr<float>() : nullptr, lse_p, n_pages, stream));
   } else if (on_tc) {
     launched("attention_prefill_tc_bounded", wpc_attention_prefill_tc_bounded(
         q.data_ptr(), q_stride, out.data_ptr(), out_stride, k.data_ptr(), v.data_ptr(), table_p, width, cu_p, ctx_p, B, max_new,
@@ -238,7 +239,7 @@ at::Tensor attention(const Args& a) {
   } else {
     launched("attention_prefill_bounded", wpc_attention_prefill_bounded(
         q.data_ptr(), q_stride, out.data_ptr(), out_stride, k.data_ptr(), v.data_ptr(), table_p, width, cu_p, ctx_p, B, max_new,
-        nh, nkv, hd, scale, window, sinks, lse_p, stream));
+        nh, nkv, hd, scale, window, sinks, lse_p, n_pages, stream));
   }
   if (!sums) return out;
   if (on_tc) {

@@ -952,7 +952,7 @@ def attention_plain(q, n_heads, n_kv_heads, head_dim, k_pages, v_pages, page_tab
     _check("attention_plain", library().wpc_attention_plain_bounded(
         _p(q), q.stride(0), _p(out), out.stride(0), _code(q.dtype), _p(k_pages), _p(v_pages), _p(page_table),
         page_table.shape[1], _p(seq_of_token), _p(positions), T, n_heads, n_kv_heads, head_dim,
-        ctypes.c_float(scale), int(window or 0), int(sinks), int(splits), _p(part), _p(lse), _stream()))
+        ctypes.c_float(scale), int(window or 0), int(sinks), int(splits), _p(part), _p(lse), k_pages.shape[0], _stream()))
     return out
 
 
