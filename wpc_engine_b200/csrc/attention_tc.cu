@@ -74,11 +74,17 @@ struct WsCfg {
   static constexpr int SMEM = 896 + NT * C::Q_BYTES + 2 * NS * C::PAGE_BYTES + N_BARS * 8 + 8;
 };
 
-// SINKS: beside its window a query sees the first `sinks` positions.  Their pages that lie before
-// the window's first page come first; pages are counted in one range (see attention_mma.cuh).
-// lse, if given, gets each row's maximum + log2(sum) in units of log 2, for the sums of weights
-// (attention_sums.cu).
-template <int HD, int NT, bool SINKS>
+// Three forms, compiled on their own (the ordinary one carries nothing of the others; with their code
+// behind run-time tests prefill of 8,192 tokens lost 2 %):
+//   PF_PLAIN  all earlier positions, or a window of them
+//   PF_SINKS  beside its window a query sees the first `sinks` positions.  Their pages that lie before
+//             the window's first page come first; pages are counted in one range (attention_mma.cuh)
+//   PF_SUMS   lse gets each row's maximum + log2(sum) in units of log 2, for the sums of weights
+//             (attention_sums_tc.cu)
+__device__ __forceinline__ uint32_t low_bits(int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1u; }
+constexpr int PF_PLAIN = 0, PF_SINKS = 1, PF_SUMS = 2;
+
+template <int HD, int NT, int MODE>
 __global__ void __launch_bounds__(WsCfg<HD, NT>::THREADS, NT == 2 ? 1 : 2)
 prefill_ws_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                   const __nv_bfloat16* __restrict__ q, int q_stride, __nv_bfloat16* __restrict__ out, int out_stride,
@@ -88,6 +94,7 @@ prefill_ws_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
                   int sinks, float* __restrict__ lse) {
   using C = Cfg<HD>;
   using W = WsCfg<HD, NT>;
+  constexpr bool SINKS = MODE == PF_SINKS;
   constexpr int NS = W::NS;
   constexpr int TROWS = NT * ROWS;
   if (!late_trigger) pdl_trigger();
@@ -297,11 +304,25 @@ prefill_ws_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
           mx4[2] = fmaxf(fmaxf(mx4[2], __uint_as_float(su[i + 4])), __uint_as_float(su[i + 5]));
           mx4[3] = fmaxf(fmaxf(mx4[3], __uint_as_float(su[i + 6])), __uint_as_float(su[i + 7]));
         }
+      } else if (MODE != PF_PLAIN) {
+        // (the keys that are seen as bits: with three comparisons a score PF_SINKS needed every register
+        // and spilled; 157 against 143 us at 2,048 tokens of 8 Ki, window 4,096)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int k0 = abs0 + h * 32;
+          const uint32_t seen = valid ? low_bits(p_row - k0 + 1) & (~low_bits(lo_row - k0) | (SINKS ? low_bits(sinks - k0) : 0u)) : 0u;
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            const float sc = seen >> i & 1 ? __uint_as_float(su[h * 32 + i]) : -INFINITY;
+            su[h * 32 + i] = __float_as_uint(sc);
+            mx4[i & 3] = fmaxf(mx4[i & 3], sc);
+          }
+        }
       } else {
 #pragma unroll
         for (int i = 0; i < 64; ++i) {
           const int kabs = abs0 + i;
-          const float sc = (valid && (kabs >= lo_row || (SINKS && kabs < sinks)) && kabs <= p_row) ? __uint_as_float(su[i]) : -INFINITY;
+          const float sc = (valid && kabs >= lo_row && kabs <= p_row) ? __uint_as_float(su[i]) : -INFINITY;
           su[i] = __float_as_uint(sc);
           mx4[i & 3] = fmaxf(mx4[i & 3], sc);
         }
@@ -359,7 +380,7 @@ prefill_ws_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
       // are issued after this page's P V and run after it.
       tmem_st32(tmem_S(t, bb) + lane_off, pw);
       tmem_st_wait();
-      if ((SINKS || lse) && abs0 + PAGE > L) {
+      if (MODE != PF_PLAIN && abs0 + PAGE > L) {
         // behind the end of the sequence lies what the page's last owner left: a weight of zero
         // times an infinity would be no zero, so those value rows are cleared before P V
         ok = mbar_wait(v_full + j % NS, (j / NS) & 1, wait_ns);
@@ -382,7 +403,7 @@ prefill_ws_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     if (!ok) atomicExch(failed, 1);
     if (ok) {
       const float inv = l_sum > 0.f ? 1.f / l_sum : 0.f;
-      if (lse && valid) lse[(size_t)(tok0 + t_row) * nh + h_row] = m_used + log2f(l_sum);
+      if (MODE == PF_SUMS && valid) lse[(size_t)(tok0 + t_row) * nh + h_row] = m_used + log2f(l_sum);
       __nv_bfloat16* dst = out + (size_t)(tok0 + t_row) * out_stride + (size_t)h_row * HD;
 #pragma unroll
       for (int c = 0; c < HD; c += 32) {
@@ -419,14 +440,14 @@ prefill_ws_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
   }
 }
 
-template <int HD, int NT, bool SINKS = false>
+template <int HD, int NT, int MODE = PF_PLAIN>
 static int launch_ws(const void* q, int q_stride, void* out, int out_stride, const void* k_pages, const void* v_pages,
                      int n_pages, const int* page_table, int table_width, const int* cu_seqlens, const int* ctx_lens,
                      int B, int max_new, int nh, int nkv, float scale, int window, int* status, cudaStream_t stream,
                      int sinks = 0, float* lse = nullptr) {
   using W = WsCfg<HD, NT>;
   static int configured[MAX_DEVICES];
-  if (int rc = allow_smem(prefill_ws_kernel<HD, NT, SINKS>, W::SMEM, configured)) return rc;
+  if (int rc = allow_smem(prefill_ws_kernel<HD, NT, MODE>, W::SMEM, configured)) return rc;
   // the cache as a matrix [n_pages * nkv * PAGE, HD]: a page of one KV head is 64 of its rows
   const long rows = (long)n_pages * nkv * PAGE;
   if (rows > 0x7fffffffL) return WPC_ERR_TOO_LARGE;
@@ -437,7 +458,7 @@ static int launch_ws(const void* q, int q_stride, void* out, int out_stride, con
   if (rc) return rc;
   const int n_rep = nh / nkv;
   dim3 grid(nkv, (max_new * n_rep + NT * ROWS - 1) / (NT * ROWS), B);
-  wpc::launch(prefill_ws_kernel<HD, NT, SINKS>, grid, W::THREADS, W::SMEM, stream, mk, mv, (const __nv_bfloat16*)q, q_stride,
+  wpc::launch(prefill_ws_kernel<HD, NT, MODE>, grid, W::THREADS, W::SMEM, stream, mk, mv, (const __nv_bfloat16*)q, q_stride,
               (__nv_bfloat16*)out, out_stride, page_table, table_width, cu_seqlens, ctx_lens, nh, nkv, scale * LOG2E,
               window, status, wait_policy().limit_ns, wait_policy().starve, NT == 1 ? sm_count() : 1 << 30,
               max_new >= 1024 ? 1 : 0, sinks, lse);
@@ -490,15 +511,16 @@ int wpc_attention_prefill_tc_bounded(const void* q, int q_stride, void* out, int
   if (!wpc_attention_prefill_tc_supports(nh, nkv, hd) || (q_stride % 8) || (out_stride % 8) ||
       (((uintptr_t)q | (uintptr_t)out | (uintptr_t)k_pages | (uintptr_t)v_pages) & 15))
     return WPC_ERR_UNSUPPORTED;
-  if (sinks < 0 || (sinks > 0 && window <= 0)) return WPC_ERR_BAD_ARGUMENT;
-#define WPC_WS(HD_, SINKS_)                                                                                          \
-  return wpc::fatc::launch_ws<HD_, 1, SINKS_>(q, q_stride, out, out_stride, k_pages, v_pages, n_pages, page_table,  \
+  if (lse ? (window > 0 || sinks != 0) : (sinks < 1 || window < 1)) return WPC_ERR_BAD_ARGUMENT;
+#define WPC_WS(HD_, MODE_)                                                                                           \
+  return wpc::fatc::launch_ws<HD_, 1, MODE_>(q, q_stride, out, out_stride, k_pages, v_pages, n_pages, page_table,  \
                                               table_width, cu_seqlens, ctx_lens, B, max_new, nh, nkv, scale, window, \
                                               status, stream, sinks, lse)
-  if (hd == 128 && sinks) WPC_WS(128, true);
-  if (hd == 128) WPC_WS(128, false);
-  if (sinks) WPC_WS(64, true);
-  WPC_WS(64, false);
+  using namespace wpc::fatc;
+  if (hd == 128 && sinks) WPC_WS(128, PF_SINKS);
+  if (hd == 128) WPC_WS(128, PF_SUMS);
+  if (sinks) WPC_WS(64, PF_SINKS);
+  WPC_WS(64, PF_SUMS);
 #undef WPC_WS
 }
 
