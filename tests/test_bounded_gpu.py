@@ -632,3 +632,57 @@ def fast_want(s):
                 w += torch.softmax((x @ k.t() * s.scale).masked_fill(at[None] > pos, -math.inf), 1).sum(0)
             sums[b, g] = w.cpu()
     return None, None, worst * (2 * hd + 4) * plain.EPS32, sums, max(s.new) * rep
+
+
+# ---- chunks of few tokens over long caches ------------------------------------------------------------
+
+CHUNKS = [([4100], [64]), ([2300, 70, 1500], [70, 3, 33]), ([700], [2]), ([1300, 1290], [130, 1])]
+
+
+@pytest.mark.parametrize("heads", [(14, 2, 64), (28, 4, 128), (3, 1, 64)])
+@pytest.mark.parametrize("lens,new", CHUNKS)
+@pytest.mark.parametrize("window,sinks", [(1000, 4), (600, 130), (5000, 1), (64, 700)])
+def test_sinks_of_chunks_over_a_long_cache(heads, lens, new, window, sinks):
+    """Row tiles whose pages are divided among several CTAs, some of which get none."""
+    s = Step(torch.bfloat16, *heads, lens, new, window, sinks, seed=window + len(lens))
+    s.check_out(s.attend(sinks=sinks), s.want())
+    assert ops.device_status() == 0
+
+
+@pytest.mark.parametrize("heads", [(14, 2, 64), (28, 4, 128), (3, 1, 64)])
+@pytest.mark.parametrize("lens,new", CHUNKS)
+def test_sums_of_chunks_over_a_long_cache(heads, lens, new):
+    s = Step(torch.bfloat16, *heads, lens, new, seed=sum(lens))
+    want, told = s.want(), s.pos
+    old, _ = s.record()
+    runs = []
+    for _ in range(2):
+        sums, stored = s.record()
+        out = s.attend(weight_sums=sums, stored_positions=stored, token_positions=told)
+        runs.append((out, sums))
+    s.check_out(out, want)
+    s.check_sums(sums, stored, old, want, told)
+    assert all(torch.equal(a, b) for a, b in zip(*runs))
+    assert ops.device_status() == 0
+
+
+@pytest.mark.parametrize("sums", [False, True])
+def test_a_nan_query_of_a_chunk_makes_nans_of_its_own_row_alone(sums):
+    window, sinks = (None, 0) if sums else (1500, 4)
+    s = Step(torch.bfloat16, 14, 2, 64, [2300, 1500], [20, 33], window, sinks, seed=8)
+    kw = {} if sums else dict(sinks=sinks)
+
+    def attend():
+        if sums:
+            kw.update(zip(("weight_sums", "stored_positions"), s.record()), token_positions=s.pos)
+        return s.attend(**kw)
+
+    clean = attend()
+    n, hd, nh = s.q.shape[0], 64, 14
+    s.q[7, 3 * hd:4 * hd] = math.nan
+    got = attend().view(n, nh, hd)
+    assert bool(got[7, 3].isnan().all())
+    rest = torch.ones(n, nh, dtype=torch.bool, device=DEV)
+    rest[7, 3] = False
+    assert torch.equal(got[rest], clean.view(n, nh, hd)[rest])
+    assert ops.device_status() == 0

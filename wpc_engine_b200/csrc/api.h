@@ -94,11 +94,13 @@ int wpc_attention_prefill_tc(const void* q, int q_stride, void* out, int out_str
                              const int* ctx_lens, int B, int max_new, int nh, int nkv, int hd, float scale,
                              int window, int* status, int n_pages, int tiles, cudaStream_t stream);
 
+// n_splits CTAs share a row tile's pages (1: none, part unused); part: float32 [n_splits * tiles * 128 * (hd + 2)]
+// with tiles = ceil(max_new * nh / nkv / 128) * nkv * B
 int wpc_attention_prefill_tc_bounded(const void* q, int q_stride, void* out, int out_stride, const void* k_pages,
                                      const void* v_pages, const int* page_table, int table_width,
                                      const int* cu_seqlens, const int* ctx_lens, int B, int max_new, int nh, int nkv,
                                      int hd, float scale, int window, int sinks, float* lse, int* status, int n_pages,
-                                     cudaStream_t stream);
+                                     int n_splits, float* part, cudaStream_t stream);
 
 // Attention with sinks beside a window (sinks > 0, window > 0), or over all earlier positions with what
 // the sums of weights need (window = 0, sinks = 0, scores, row_ml / lse given): attention_bounded.cu.

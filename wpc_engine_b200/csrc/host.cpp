@@ -233,9 +233,19 @@ at::Tensor attention(const Args& a) {
         width, seq.data_ptr<int>(), pos.data_ptr<int>(), T, nh, nkv, hd, scale, window, sinks, splits,
         splits > 1 ? part.data_ptr<float>() : nullptr, lse_p, n_pages, stream));
   } else if (on_tc) {
+    // A chunk of few tokens over a long cache has fewer row tiles than the SMs have places (two each): then as
+    // many CTAs as there are places for share a tile's pages, four pages each at least.  7B shape:
+    // 64 tokens of 2,048 positions, window 1,024: alone 23.0 us, 4 pages each 14.4, 8 pages 18.0; of 8,192, window
+    // 4,096: 64.0, 23.0, 19.1 (two tokens: 68.8, 16.5, 18.0); 512 tokens (two CTAs to a tile) 63.8 -> 48.1, and with
+    // the shorter window 24.2 -> 24.6.
+    const long tiles = ((long)max_new * (nh / nkv) + 127) / 128 * nkv * B;
+    const long seen = window ? std::min<long>(max_ctx, (long)window + max_new + sinks + PAGE) : max_ctx;
+    const int splits = (int)std::max<long>(1, std::min<long>(std::min<long>(16, 2L * n_sms / tiles), seen / PAGE / 4));
+    at::Tensor part;
+    if (splits > 1) part = empty({splits * tiles * 128 * (hd + 2)}, at::kFloat, device);
     launched("attention_prefill_tc_bounded", wpc_attention_prefill_tc_bounded(
         q.data_ptr(), q_stride, out.data_ptr(), out_stride, k.data_ptr(), v.data_ptr(), table_p, width, cu_p, ctx_p, B, max_new,
-        nh, nkv, hd, scale, window, sinks, lse_p, status, n_pages, stream));
+        nh, nkv, hd, scale, window, sinks, lse_p, status, n_pages, splits, splits > 1 ? part.data_ptr<float>() : nullptr, stream));
   } else {
     launched("attention_prefill_bounded", wpc_attention_prefill_bounded(
         q.data_ptr(), q_stride, out.data_ptr(), out_stride, k.data_ptr(), v.data_ptr(), table_p, width, cu_p, ctx_p, B, max_new,
