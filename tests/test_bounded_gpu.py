@@ -686,3 +686,36 @@ def test_a_nan_query_of_a_chunk_makes_nans_of_its_own_row_alone(sums):
     rest[7, 3] = False
     assert torch.equal(got[rest], clean.view(n, nh, hd)[rest])
     assert ops.device_status() == 0
+
+
+# ---- steps with sequences that bring nothing, bounds larger than the step -----------------------------------
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("heads", [(14, 2, 64), (28, 4, 128), (4, 2, 48)])
+@pytest.mark.parametrize("sums", [False, True])
+@pytest.mark.parametrize("new", [[5, 0, 0, 70, 0], [0, 1, 0, 1, 0], [0, 1, 0, 0, 0]])
+def test_sequences_without_new_tokens_and_a_bound_larger_than_any(dtype, heads, sums, new):
+    window, sinks = (None, 0) if sums else (100, 4)
+    s = Step(dtype, *heads, [130, 65, 0, 300, 64], new, window, sinks, seed=12)
+    want, told = s.want(), s.pos + 3
+    s.max_new = 1 << 30                   # (the kernels' grids go by the tokens that are there)
+    old, _ = s.record()
+    sums_now, stored = s.record()
+    kw = dict(weight_sums=sums_now, stored_positions=stored, token_positions=told) if sums else dict(sinks=sinks)
+    got = s.attend(**kw)
+    s.check_out(got, want)
+    if sums:
+        s.check_sums(sums_now, stored, old, want, told)
+    assert ops.device_status() == 0
+
+
+def test_refusals_of_sizes_that_do_not_go_together():
+    s = Step(torch.bfloat16, 14, 2, 64, [300, 70], [3, 1], 100, 4, seed=1)
+    no = ints([])
+    for new in (1, 3):
+        with pytest.raises(ops.KernelError, match="no sequences"):
+            ops.attention(s.q, *s.heads, s.k, s.v, s.table[:0], ints([0]), no, s.seq, s.pos, s.scale, 100, new, 300, sinks=4)
+        for heads in ((14, 0), (13, 2)):
+            with pytest.raises(ops.KernelError, match="multiple of n_kv_heads"):
+                ops.attention(s.q, *heads, 64, s.k, s.v, s.table, s.cu, s.ctx, s.seq, s.pos, s.scale, 100, new, 300, sinks=4)
+    assert ops.device_status() == 0

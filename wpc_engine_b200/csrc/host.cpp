@@ -171,6 +171,7 @@ at::Tensor attention(const Args& a) {
   }
   at::Tensor out = empty({T, (long)nh * hd}, type, device);
   if (T == 0) return out;
+  if (B < 1) refuse("q has tokens, but there are no sequences");
   const cudaStream_t stream = c10::cuda::getCurrentCUDAStream(device).stream();
   const int n_sms = as_int(a.number(23), "n_sms");
   int* const status = (int*)a.tensor(24, "status").data_ptr();
@@ -209,6 +210,7 @@ at::Tensor attention(const Args& a) {
         row_ml, told, max_ctx, n_pages, weight_sums, stored, status, stream));
     return out;
   }
+  const int longest = std::min(max_new, T);              // (a larger bound would only start blocks without work)
   at::Tensor lse;
   float* lse_p = nullptr;
   if (sums) {
@@ -238,17 +240,17 @@ at::Tensor attention(const Args& a) {
     // 64 tokens of 2,048 positions, window 1,024: alone 23.0 us, 4 pages each 14.4, 8 pages 18.0; of 8,192, window
     // 4,096: 64.0, 23.0, 19.1 (two tokens: 68.8, 16.5, 18.0); 512 tokens (two CTAs to a tile) 63.8 -> 48.1, and with
     // the shorter window 24.2 -> 24.6.
-    const long tiles = ((long)max_new * (nh / nkv) + 127) / 128 * nkv * B;
-    const long seen = window ? std::min<long>(max_ctx, (long)window + max_new + sinks + PAGE) : max_ctx;
+    const long tiles = ((long)longest * (nh / nkv) + 127) / 128 * nkv * B;
+    const long seen = window ? std::min<long>(max_ctx, (long)window + longest + sinks + PAGE) : max_ctx;
     const int splits = (int)std::max<long>(1, std::min<long>(std::min<long>(16, 2L * n_sms / tiles), seen / PAGE / 4));
     at::Tensor part;
     if (splits > 1) part = empty({splits * tiles * 128 * (hd + 2)}, at::kFloat, device);
     launched("attention_prefill_tc_bounded", wpc_attention_prefill_tc_bounded(
-        q.data_ptr(), q_stride, out.data_ptr(), out_stride, k.data_ptr(), v.data_ptr(), table_p, width, cu_p, ctx_p, B, max_new,
+        q.data_ptr(), q_stride, out.data_ptr(), out_stride, k.data_ptr(), v.data_ptr(), table_p, width, cu_p, ctx_p, B, longest,
         nh, nkv, hd, scale, window, sinks, lse_p, status, n_pages, splits, splits > 1 ? part.data_ptr<float>() : nullptr, stream));
   } else {
     launched("attention_prefill_bounded", wpc_attention_prefill_bounded(
-        q.data_ptr(), q_stride, out.data_ptr(), out_stride, k.data_ptr(), v.data_ptr(), table_p, width, cu_p, ctx_p, B, max_new,
+        q.data_ptr(), q_stride, out.data_ptr(), out_stride, k.data_ptr(), v.data_ptr(), table_p, width, cu_p, ctx_p, B, longest,
         nh, nkv, hd, scale, window, sinks, lse_p, n_pages, stream));
   }
   if (!sums) return out;
@@ -257,17 +259,17 @@ at::Tensor attention(const Args& a) {
     const long n_tickets = (long)B * nkv * ((max_ctx + SUMS_KEYS - 1) / SUMS_KEYS);
     at::Tensor tickets = tickets_of(n_tickets, device, stream);
     launched("weight_sums_tc", wpc_weight_sums_tc(
-        q.data_ptr(), q_stride, T, k.data_ptr(), table_p, width, cu_p, ctx_p, told, lse_p, B, nh, nkv, hd, scale, max_new,
+        q.data_ptr(), q_stride, T, k.data_ptr(), table_p, width, cu_p, ctx_p, told, lse_p, B, nh, nkv, hd, scale, longest,
         max_ctx, n_pages, weight_sums, stored, status, part.data_ptr<float>(), tickets.data_ptr<int>(), (int)tickets.numel(),
         stream));
   } else if (aligned) {
     launched("weight_sums_mma", wpc_weight_sums_mma(
-        q.data_ptr(), q_stride, k.data_ptr(), table_p, width, cu_p, ctx_p, told, lse_p, B, nh, nkv, hd, scale, max_new, max_ctx,
+        q.data_ptr(), q_stride, k.data_ptr(), table_p, width, cu_p, ctx_p, told, lse_p, B, nh, nkv, hd, scale, longest, max_ctx,
         n_pages, weight_sums, stored, status, stream));
   } else {
     launched("weight_sums_plain", wpc_weight_sums_plain(
         q.data_ptr(), q_stride, type == at::kFloat ? 0 : 1, k.data_ptr(), table_p, width, cu_p, ctx_p, told, lse_p, B, nh, nkv,
-        hd, scale, max_new, max_ctx, n_pages, weight_sums, stored, status, stream));
+        hd, scale, longest, max_ctx, n_pages, weight_sums, stored, status, stream));
   }
   return out;
 }

@@ -746,6 +746,8 @@ def attention(q: torch.Tensor, n_heads: int, n_kv_heads: int, head_dim: int, k_p
 @functools.lru_cache(maxsize=4096)
 def _bounded_decode_plan(n_seqs, n_kv_heads, n_heads, head_dim, blocks, splits, cluster, groups, n_sms):
     """(cluster, groups, n_ctas) of a decode step in which a query sees `blocks` pages."""
+    if n_kv_heads < 1 or n_heads % n_kv_heads:
+        raise KernelError(f"n_heads must be a multiple of n_kv_heads, got {n_heads} and {n_kv_heads}")
     ctx = blocks * PAGE
     if cluster is None:
         cluster, groups = (0, 1) if splits else plan_decode_cluster(n_seqs, n_kv_heads, n_heads, head_dim, ctx, None)
@@ -928,20 +930,17 @@ def plan_decode_cluster(n_seqs: int, n_kv_heads: int, n_heads: int, head_dim: in
 
 
 def attention_plain(q, n_heads, n_kv_heads, head_dim, k_pages, v_pages, page_table, seq_of_token, positions,
-                    scale, window, max_ctx_len: Optional[int] = None, splits: Optional[int] = None, sinks: int = 0,
-                    lse: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+                    scale, window, max_ctx_len: Optional[int] = None, splits: Optional[int] = None, sinks: int = 0) -> torch.Tensor:
     """The attention of the 32-bit path and the plain twin of the fast kernels: a block to each
     (token, head).  With few tokens and long contexts (`max_ctx_len`, the longest sequence of
     the step) several blocks share a query's keys, about 256 each and no more blocks than fill
     the device twice (`splits` forces their number); their parts are added in order.  `sinks`: see
-    `attention`; `lse` (float32 [T, n_heads]) gets maximum + log2(sum) of each row's scores in
-    units of log 2; `out`: where the result goes (contiguous)."""
+    `attention`."""
     _rows(q, "q")
     _need(q.shape[1] >= n_heads * head_dim, "q is too narrow")
     _need(k_pages.is_contiguous() and v_pages.is_contiguous() and k_pages.dtype == q.dtype, "pages: wrong type")
     T = q.shape[0]
-    if out is None:
-        out = torch.empty((T, n_heads * head_dim), dtype=q.dtype, device=q.device)
+    out = torch.empty((T, n_heads * head_dim), dtype=q.dtype, device=q.device)
     sinks = sinks if window else 0
     if splits is None:
         keys = min(max_ctx_len or 0, window + sinks if window else (max_ctx_len or 0))
@@ -952,7 +951,7 @@ def attention_plain(q, n_heads, n_kv_heads, head_dim, k_pages, v_pages, page_tab
     _check("attention_plain", library().wpc_attention_plain_bounded(
         _p(q), q.stride(0), _p(out), out.stride(0), _code(q.dtype), _p(k_pages), _p(v_pages), _p(page_table),
         page_table.shape[1], _p(seq_of_token), _p(positions), T, n_heads, n_kv_heads, head_dim,
-        ctypes.c_float(scale), int(window or 0), int(sinks), int(splits), _p(part), _p(lse), k_pages.shape[0], _stream()))
+        ctypes.c_float(scale), int(window or 0), int(sinks), int(splits), _p(part), None, k_pages.shape[0], _stream()))
     return out
 
 
