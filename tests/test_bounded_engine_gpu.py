@@ -161,3 +161,17 @@ def test_the_command_line_takes_a_bounded_cache(tmp_path):
     assert len(tokens) == 60 and tokens == generate(eng, [ids(200)], GenerationOptions(max_tokens=60))[0]
     refused = run("--cache-keep", "10", "--cache-recent", "9")
     assert refused.returncode == 2 and "does not hold" in refused.stderr
+
+
+def test_the_command_line_prints_logits_of_prompts_longer_than_a_step(tmp_path):
+    folder = folder_of(tmp_path, WIDE, torch.float32)
+    base = [sys.executable, os.path.join(ROOT, "bin", "wpc-runtime"), "--model", folder, "--dtype", "fp32", "--prompt-ids",
+            ",".join(map(str, ids(100))), "--max-tokens", "2", "--stop-ids", "", "--print-logits", "1"]
+    run = lambda *more: subprocess.run(base + list(more), capture_output=True, text=True, timeout=300)   # noqa: E731
+    whole, parts = run(), run("--max-step-tokens", "30")
+    assert whole.returncode == 0 and parts.returncode == 0, parts.stderr
+    (a, b), (c, d) = ([json.loads(line) for line in r.stdout.splitlines()] for r in (whole, parts))
+    assert a["top_logits"][0][0] == c["top_logits"][0][0] and b == d
+    for more, word in ((("--max-step-tokens", "0"), "at least 1"), (("--cache-recent", "5"), "--cache-keep")):
+        refused = run(*more)
+        assert refused.returncode == 2 and word in refused.stderr

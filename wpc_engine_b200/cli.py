@@ -88,6 +88,12 @@ def main(argv=None) -> int:
         write_random_model(args.model, cfg, args.seed, torch.bfloat16 if dtype == "bfloat16" else torch.float32)
         print(f"wrote random weights (seed {args.seed}) to {args.model}", file=sys.stderr)
 
+    if args.max_step_tokens is not None and args.max_step_tokens < 1:
+        print(f"error: --max-step-tokens must be at least 1, got {args.max_step_tokens}", file=sys.stderr)
+        return 2
+    if args.cache_keep is None and args.cache_recent is not None:
+        print("error: --cache-recent is a part of --cache-keep, which is not given", file=sys.stderr)
+        return 2
     eviction = None
     if args.cache_keep is not None:
         recent = args.cache_keep // 4 if args.cache_recent is None else args.cache_recent
@@ -126,11 +132,13 @@ def main(argv=None) -> int:
     if stop:
         print(f"stop tokens: {stop}", file=sys.stderr)
     if args.print_logits > 0:
-        from . import SequenceStep
+        from .engine.generate import prompt_steps
         for i, p in enumerate(prompts):
             slot = engine.open_sequence()
             try:
-                row = engine.step([SequenceStep(slot, p, want=[len(p) - 1])])[0].float()
+                for step in prompt_steps([slot], [p], engine.max_step_tokens):
+                    logits = engine.step(step)
+                row = logits[0].float()
             finally:
                 engine.close_sequence(slot)
             vals, ids = torch.topk(row, min(args.print_logits, row.numel()))

@@ -188,7 +188,8 @@ class Engine:
         `check` (default: the engine's `check_status`): read the device error word after the
         step, which waits for the device, and raise `KernelError` if a kernel of the step gave
         up.  A step that raises, for whatever reason, leaves the sequences as they were: the
-        pages that it had taken go back."""
+        pages that it had taken go back.  (With eviction a step that a kernel gave up in may have added
+        to the sums of entries stored before it.)"""
         self._check(entries)
         reserved = []
         try:

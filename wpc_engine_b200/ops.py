@@ -762,16 +762,18 @@ def _bounded_attention(q, n_heads, n_kv_heads, head_dim, k_pages, v_pages, page_
     global launch_count
     if not q.is_cuda:
         raise KernelError("q must be on a CUDA device")
-    n_ctas, n_sms = 0, _sms_of.get(q.get_device()) or sms()
+    device = q.get_device()
+    n_ctas, n_sms = 0, _sms_of.get(device) or sms()
     if max_new_tokens == 1:
         blocks = -(-max_ctx_len // PAGE)
         if window:
             blocks = min(blocks, -(-window // PAGE) + 1 + -(-sinks // PAGE))
         cluster, groups, n_ctas = _bounded_decode_plan(ctx_lens.numel(), n_kv_heads, n_heads, head_dim, blocks, splits, cluster,
                                                        groups, n_sms)
-    out = host().attention(q, n_heads, n_kv_heads, head_dim, k_pages, v_pages, page_table, cu_seqlens, ctx_lens, seq_of_token,
-                           positions, scale, window or 0, max_new_tokens, max_ctx_len, mma_only, sinks, weight_sums,
-                           stored_positions, token_positions, cluster or 0, groups, n_ctas, n_sms, workspace(q.device)[2])
+    out = (_host or host()).attention(
+        q, n_heads, n_kv_heads, head_dim, k_pages, v_pages, page_table, cu_seqlens, ctx_lens, seq_of_token, positions, scale,
+        window or 0, max_new_tokens, max_ctx_len, mma_only, sinks, weight_sums, stored_positions, token_positions,
+        cluster or 0, groups, n_ctas, n_sms, (_workspaces.get(device) or workspace(q.device))[2])
     launch_count += 1 if weight_sums is None else 2
     return out
 
