@@ -659,6 +659,11 @@ decode_cluster_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, __nv_bf
     cp_async_commit();
   }
   pdl_wait();
+  // (the query first: its loads cannot be moved across the copies)
+  const int r_lo = lane >> 2, r_hi = r_lo + 8;                        // rows = heads of the group
+  const __nv_bfloat16* qtok = after_wait(q) + (size_t)b * q_stride + (size_t)g * n_rep * HD;
+  uint32_t qf[HD / 16][4];
+  load_q<HD>(qf, r_lo < n_rep ? qtok + r_lo * HD : nullptr, r_hi < n_rep ? qtok + r_hi * HD : nullptr, lane);
   for (int i = filled; i < DECODE_STAGES - 1; ++i) {
     if (blk0 + i < blk1) {
       const size_t src = (size_t)max(page_of(blk0 + i), 0) * page_elems + (size_t)g * PAGE * HD;
@@ -667,10 +672,6 @@ decode_cluster_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, __nv_bf
     }
     cp_async_commit();
   }
-  const int r_lo = lane >> 2, r_hi = r_lo + 8;                        // rows = heads of the group
-  const __nv_bfloat16* qtok = after_wait(q) + (size_t)b * q_stride + (size_t)g * n_rep * HD;
-  uint32_t qf[HD / 16][4];
-  load_q<HD>(qf, r_lo < n_rep ? qtok + r_lo * HD : nullptr, r_hi < n_rep ? qtok + r_hi * HD : nullptr, lane);
   float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
   float o[HD / 8][4];
 #pragma unroll

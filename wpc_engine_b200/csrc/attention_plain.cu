@@ -15,13 +15,6 @@ namespace wpc {
 
 constexpr int AP_THREADS = 128;
 
-// four consecutive elements of a key row as floats (the row starts 16-byte aligned when hd is a multiple of 4)
-__device__ __forceinline__ float4 load4(const float* p) { return *(const float4*)p; }
-__device__ __forceinline__ float4 load4(const __nv_bfloat16* p) {
-  const uint2 t = *(const uint2*)p;
-  const float2 a = __bfloat1622float2(*(const __nv_bfloat162*)&t.x), b = __bfloat1622float2(*(const __nv_bfloat162*)&t.y);
-  return make_float4(a.x, a.y, b.x, b.y);
-}
 constexpr int AP_CHUNK = 512;        // keys per chunk; their scores live in shared memory
 
 template <typename T>

@@ -26,7 +26,7 @@
 //   s_empty[2][2]             threads -> MMA     they have been read (128 arrivals)
 //
 // Bound by the exponentials: a prompt of 2,048 tokens of the 7B shape (28 heads, 4 KV heads of 128) has 59
-// million, 15.7 us at the unit's rate of 16 a cycle and SM; the kernel takes 26 of the call's 71 us, of
+// million, 15.7 us at the unit's rate of 16 a cycle and SM; the kernel takes 26 of the call's 69 us, of
 // which 8 are the start, the first keys and the tickets (30 of 76 with the copies started after tensor
 // memory was there).  A CTA to a key tile, with the queries shared in clusters, instead of equal shares of the list:
 // 42.  An eighth or three of the exponentials by a polynomial changed nothing (76.4 and 75.4).

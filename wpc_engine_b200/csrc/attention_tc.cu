@@ -281,11 +281,13 @@ prefill_ws_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     {
       const __nv_bfloat16* src = after_wait(q) + (size_t)(tok0 + t_row) * q_stride + (size_t)h_row * HD;
       uint8_t* my_q = base + t * C::Q_BYTES;
+      // (all loads ahead of the first store, which they cannot be moved across: 2,048 tokens of the 7B shape
+      // 41.4 -> 39.6 us, 16 prompts of 512 of the 0.5B shape 42.5 -> 37.7)
+      uint4 v[HD / 8];
 #pragma unroll
-      for (int c = 0; c < HD / 8; ++c) {
-        uint4 v = valid ? *(const uint4*)(src + c * 8) : make_uint4(0, 0, 0, 0);
-        *(uint4*)(my_q + (c >> 3) * (ROWS * 128) + swz(rt, c & 7)) = v;
-      }
+      for (int c = 0; c < HD / 8; ++c) v[c] = valid ? *(const uint4*)(src + c * 8) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int c = 0; c < HD / 8; ++c) *(uint4*)(my_q + (c >> 3) * (ROWS * 128) + swz(rt, c & 7)) = v[c];
       fence_async_smem();
       mbar_arrive(q_full);
     }
@@ -470,8 +472,8 @@ prefill_ws_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
 
 // Joins the shares of a row tile: a thread to a row and JOIN of its values.  Reads what the shares wrote, from L2,
 // 16 bytes a thread with a warp's rows side by side (outputs laid out by rows instead: 512 tokens in two shares
-// 29.8 us against 24.6); with one share's loads at a time the join of 16 shares took 5 us longer.  Grid as the shared kernel's, with
-// HD / JOIN blocks to a tile in place of its shares.
+// 29.8 us against 24.6); with one share's loads at a time the join of 16 shares took 5 us longer.  Grid as the
+// shared kernel's, with HD / JOIN blocks to a tile in place of its shares.
 constexpr int JOIN = 16;
 template <int HD>
 __global__ void __launch_bounds__(ROWS)
