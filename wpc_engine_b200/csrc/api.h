@@ -15,7 +15,8 @@ int wpc_set_pdl(int on);
 // How long a kernel waits on one of its mbarriers before it gives up, records
 // WPC_ERR_DEVICE_WAIT in the status word it was given and returns (default 2 s).  `starve` = 1
 // is for tests of that path: the kernels with TMA producers start no copies, so their waits
-// run out; nothing else about them changes.
+// run out; nothing else about them changes.  2: the same, but in the kernel of prompts' weight
+// sums in every other CTA only.
 int wpc_set_wait_policy(unsigned long long limit_ns, int starve);
 
 int wpc_embed(const int* tokens, const void* table, int table_dtype, float* out, int T, int H, int V,

@@ -13,7 +13,9 @@
 // (sequence, key tile, KV head) each, so that every SM does the same number of exponentials,
 // whatever the lengths.  A segment that holds all query tiles of its keys adds their sums itself; the
 // others leave theirs in scratch memory, and the CTA that takes the keys' last ticket adds them
-// in the order of the list (the same bits every run; nobody waits).
+// in the order of the list (the same bits every run; nobody waits).  A CTA whose wait ran out still takes the
+// tickets of all its segments, with a mark, so that they are zero again for the next launch; marked keys
+// get no sum.
 //
 // A query tile is as many whole tokens as fit 128 rows (18 of 7 heads): one 3D TMA box of
 // [tokens][heads of the group][64] elements for each 64-wide half of a head.  Warps 0..7 add (four for
@@ -45,6 +47,7 @@ constexpr int ST_KEYS = 256;             // keys of a segment: four pages
 constexpr int ST_COLS = 128;             // (token, head) rows of a query tile, padded
 constexpr int ST_THREADS = 320;
 constexpr int ST_MMA_WARP = 8, ST_COPY_WARP = 9;
+constexpr int ST_FAILED = 1 << 16;       // in a ticket: a CTA's wait ran out (the count below it: at most the CTAs of a grid)
 
 template <int HD>
 struct StCfg {
@@ -270,7 +273,7 @@ prefill_sums_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
   sg.n = min(sg.all - sg.t0, sg.left);
   sg.load(work);
 
-  const bool copies = warp == ST_COPY_WARP && lane == 0 && !starve;
+  const bool copies = warp == ST_COPY_WARP && lane == 0 && !(starve == STARVE_ODD ? blockIdx.x & 1 : starve);
   // the copies of a segment's keys, and of its j-th query tile (number i since the kernel's start)
   auto copy_keys = [&](int s) {
     const int* table = t.page_table + (size_t)sg.b * t.table_width;
@@ -427,25 +430,30 @@ prefill_sums_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
         }
       }
       float w = ((acc[0].x + acc[0].y) + (acc[1].x + acc[1].y)) + ((acc[2].x + acc[2].y) + (acc[3].x + acc[3].y));
-      // ---- the end of a segment (both halves meet here, whatever became of their waits) ----
+      // ---- the end of a segment (both halves meet here, whatever became of their waits; after one that ran
+      // out the CTA walks the rest of its share without waiting or adding, for the tickets alone) ----
+      bool adds;
       if (sg.n == sg.all) {
-        if (!all_of(3, 256, ok)) { ok = false; break; }
+        adds = ok = all_of(3, 256, ok);
       } else {
         // The keys' units are [first, first + all): this CTA's part goes to its slot 0 if it is the
         // first segment of its share, else to slot 1 (it is the last one then).
         const int first = sg.unit - sg.t0;
         part[(size_t)(2 * blockIdx.x + (sg.unit == u0 ? 0 : 1)) * ST_KEYS + half * 128 + r] = w;
         __threadfence();
-        if (!all_of(3, 256, ok)) { ok = false; break; }
+        ok = all_of(3, 256, ok);
         const int c0 = first / per, c1 = (first + sg.all - 1) / per;
         if (tid == 0) {
           int* ticket = tickets + (sg.b * work.key_tiles + sg.kt) * work.nkv + sg.g;
-          s_last = atomicAdd(ticket, 1) == c1 - c0;
-          if (s_last) *ticket = 0;                           // ready for the next launch
+          const int taken = atomicAdd(ticket, ok ? 1 : ST_FAILED + 1);
+          const bool last = (taken & (ST_FAILED - 1)) == c1 - c0;
+          if (last) *ticket = 0;                             // ready for the next launch
+          s_last = last && ok && taken < ST_FAILED;          // (with a failed CTA among them nobody adds)
           __threadfence();
         }
         all_of(3, 256, true);
-        if (s_last) {
+        adds = s_last;
+        if (adds) {
           w = 0.f;
           for (int c = c0; c <= c1; c += 8) {                // (eight loads on their way at a time)
             float v[8];
@@ -458,7 +466,7 @@ prefill_sums_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
         }
         all_of(3, 256, true);                                // (s_last is written again)
       }
-      if ((sg.n == sg.all || s_last) && key < sg.L)
+      if (adds && key < sg.L)
         add_sum(t, work.nkv, sg.b, sg.g, key, key >= sg.start ? sg.tok0 + key - sg.start : -1, w);
       more = sg.next(work);
     }

@@ -214,8 +214,10 @@ inline void launch_clusters(void (*kernel)(KArgs...), dim3 grid, dim3 block, siz
 // WPC_ERR_DEVICE_WAIT in the device status word and returns.  `starve` is a switch for tests of
 // that path: the warp that starts a kernel's TMA copies starts none, so that the barriers that
 // wait for data are never signalled and the waits run out (nothing is in flight then, nothing
-// traps, and the kernel leaves as it would after a real loss).  Both are copied into a
-// kernel's arguments at launch.
+// traps, and the kernel leaves as it would after a real loss).  STARVE_ODD does so in every other CTA
+// of the kernel of prompts' weight sums, whose CTAs share tickets (in all of the other kernels).  Both
+// are copied into a kernel's arguments at launch.
+constexpr int STARVE_ODD = 2;
 struct WaitPolicy {
   unsigned long long limit_ns;
   int starve;

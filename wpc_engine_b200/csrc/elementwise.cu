@@ -320,9 +320,9 @@ int wpc_set_pdl(int on) {
 }
 
 int wpc_set_wait_policy(unsigned long long limit_ns, int starve) {
-  if (limit_ns == 0) return WPC_ERR_BAD_ARGUMENT;
+  if (limit_ns == 0 || starve < 0 || starve > STARVE_ODD) return WPC_ERR_BAD_ARGUMENT;
   wait_policy().limit_ns = limit_ns;
-  wait_policy().starve = starve ? 1 : 0;
+  wait_policy().starve = starve;
   return 0;
 }
 

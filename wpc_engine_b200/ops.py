@@ -12,7 +12,7 @@ import ctypes
 import functools
 import os
 import threading
-from typing import Optional, Tuple
+from typing import Optional, Tuple, Union
 
 import torch
 
@@ -73,11 +73,12 @@ def host():
     return _host
 
 
-def set_wait_policy(limit_ns: int = 2_000_000_000, starve: bool = False) -> None:
+def set_wait_policy(limit_ns: int = 2_000_000_000, starve: Union[bool, int] = False) -> None:
     """How long a kernel waits on one of its barriers before it gives up and records an error
     in the device status word (2 s by default).  `starve` is for tests of that path: kernels
-    with TMA producers then start no copies, so that their waits run out."""
-    _check("set_wait_policy", library().wpc_set_wait_policy(ctypes.c_ulonglong(int(limit_ns)), int(bool(starve))))
+    with TMA producers then start no copies, so that their waits run out (2: every other CTA only in
+    the kernel of prompts' weight sums, whose CTAs share tickets)."""
+    _check("set_wait_policy", library().wpc_set_wait_policy(ctypes.c_ulonglong(int(limit_ns)), int(starve)))
 
 
 def set_pdl(on: bool) -> bool:
