@@ -48,3 +48,98 @@ def test_wait_policies_that_do_not_exist_are_refused():
     for starve in (-1, 3):
         with pytest.raises(ops.KernelError, match="bad argument"):
             ops.set_wait_policy(3_000_000, starve=starve)
+
+
+def waits(stream):
+    import ctypes
+    return bool(ops.library().wpc_pdl_next_waits(ctypes.c_void_p(stream.cuda_stream)))
+
+
+def a_move(seed=1):
+    sums, stored, table, k, v = eviction_case(2, 2, [300, 200], seed, hd=64, special=False)
+    kept = ops.select_kept(sums, stored, table, ints([300, 200]), ints([1500, 1500]), 100, 2, 30)
+    return lambda: ops.move_kept_(k, v, sums, stored, table, kept), (k, v, sums, stored, table)
+
+
+def test_the_kernel_behind_a_move_waits_on_the_moves_own_stream():
+    """Launches on other streams and from other threads in between do not use the wait up."""
+    import threading
+    move, _ = a_move()
+    x, gain = torch.ones(4, 64, device=DEV), torch.ones(64, device=DEV)
+    one, two = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+
+    def norm(stream):
+        with torch.cuda.stream(stream):
+            ops.rmsnorm(x, gain, 1e-6, torch.float32)
+
+    for s in (one, two):
+        norm(s)
+        assert not waits(s)
+    with torch.cuda.stream(one):
+        move()
+    assert waits(one) and not waits(two)
+    norm(two)
+    assert waits(one)
+    thread = threading.Thread(target=norm, args=(two,))
+    thread.start()
+    thread.join()
+    assert waits(one)
+    with torch.cuda.stream(two):
+        move()
+    thread = threading.Thread(target=norm, args=(one,))      # another thread's launch on the stream is the one that waits
+    thread.start()
+    thread.join()
+    assert not waits(one) and waits(two)
+    norm(two)
+    assert not waits(two)
+    torch.cuda.synchronize()
+
+
+def test_a_capture_does_not_use_up_the_wait_of_its_stream():
+    move, _ = a_move()
+    x, gain = torch.ones(4, 64, device=DEV), torch.ones(64, device=DEV)
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        move()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            ops.rmsnorm(x, gain, 1e-6, torch.float32)
+        assert waits(stream)
+        ops.rmsnorm(x, gain, 1e-6, torch.float32)
+        assert not waits(stream)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            move()
+            assert waits(stream)
+            ops.rmsnorm(x, gain, 1e-6, torch.float32)
+            assert not waits(stream)
+        graph.replay()
+    torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("how", [dict(cluster=0), dict(cluster=3), dict(cluster=4, groups=2)])
+def test_decode_behind_a_move_sees_what_was_moved(how):
+    """Move, a call on another stream, decode: again and again with other data."""
+    lens, keep = [900] * 8, 640
+    s = Step(torch.bfloat16, 28, 4, 128, [keep + 1] * 8, [1] * 8, seed=1)
+    sums, stored, table, k, v = eviction_case(1, 4, lens, 2, hd=128, special=False)
+    s.table, s.k, s.v = table, k[0], v[0]
+    kept = ops.select_kept(sums, stored, table, ints(lens), ints([3000] * 8), keep, 4, 50)
+    x, gain, other = torch.ones(4, 64, device=DEV), torch.ones(64, device=DEV), torch.cuda.Stream()
+    start = [t.clone() for t in (k, v, sums, stored)]
+    want = None
+    for i in range(20):
+        for t, o in zip((k, v, sums, stored), start):
+            t.copy_(o)
+        ops.move_kept_(k, v, sums, stored, table, kept)
+        if want is None:
+            torch.cuda.synchronize()
+        with torch.cuda.stream(other):
+            ops.rmsnorm(x, gain, 1e-6, torch.float32)
+        record = s.record() if want is None else (sums[0], stored[0])
+        got = s.attend(weight_sums=record[0], stored_positions=record[1], token_positions=s.pos, **how)
+        if want is None:
+            want = got.clone()
+        assert torch.equal(got, want)

@@ -12,6 +12,9 @@ extern "C" {
 
 // Programmatic dependent launch for all kernels of the library: on (1, the default) or off (0).
 int wpc_set_pdl(int on);
+// 1 if the next kernel of the library on this stream of the current device will not start ahead of the
+// one before it (after wpc_move_kept), else 0.
+int wpc_pdl_next_waits(cudaStream_t stream);
 // How long a kernel waits on one of its mbarriers before it gives up, records
 // WPC_ERR_DEVICE_WAIT in the status word it was given and returns (default 2 s).  `starve` = 1
 // is for tests of that path: the kernels with TMA producers start no copies, so their waits

@@ -4,6 +4,11 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+#include <mutex>
+#include <set>
+#include <tuple>
+
 #define WPC_DTYPE_F32 0
 #define WPC_DTYPE_BF16 1
 
@@ -159,10 +164,57 @@ inline int& pdl_enabled() {
   static int on = 1;
   return on;
 }
-// Set to 1 before a launch that should not start ahead of the kernel before it; cleared by the launch.
+// Set to 1 right before a launch that should not start ahead of the kernel before it; cleared by the launch.
 inline int& pdl_skip_next() {
   static thread_local int skip = 0;
   return skip;
+}
+// Streams whose next kernel of this library must not start ahead of the one before it, whichever thread
+// launches it: what that one wrote is read ahead of a dependency wait (decode attention reads pages so).
+// What a capture queues on a stream is another queue than the stream's own: the two count apart.
+class PdlWaiting {
+ public:
+  void add(cudaStream_t stream) {
+    const Queue q = queue(stream);
+    std::lock_guard<std::mutex> hold(lock_);
+    queues_.insert(q);
+    n_.store((int)queues_.size(), std::memory_order_release);
+  }
+  // Whether the next kernel of `stream` has to wait; take: it is being launched.
+  bool next(cudaStream_t stream, bool take) {
+    if (n_.load(std::memory_order_acquire) == 0) return false;         // (every launch asks)
+    const Queue q = queue(stream);
+    std::lock_guard<std::mutex> hold(lock_);
+    const bool waits = queues_.count(q) != 0;
+    if (waits && take) {
+      queues_.erase(q);
+      n_.store((int)queues_.size(), std::memory_order_release);
+    }
+    return waits;
+  }
+  static PdlWaiting& all() {
+    static auto* w = new PdlWaiting();                                 // (outlives the process's last launch)
+    return *w;
+  }
+
+ private:
+  using Queue = std::tuple<int, cudaStream_t, unsigned long long>;     // device, stream, capture (0: none)
+  static Queue queue(cudaStream_t stream) {
+    int device = 0;
+    cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+    unsigned long long id = 0;
+    if (cudaGetDevice(&device) != cudaSuccess) device = -1;
+    if (cudaStreamGetCaptureInfo(stream, &status, &id) != cudaSuccess || status == cudaStreamCaptureStatusNone) id = 0;
+    return {device, stream, id};
+  }
+  std::mutex lock_;
+  std::set<Queue> queues_;
+  std::atomic<int> n_{0};
+};
+inline bool pdl_allowed(cudaStream_t stream) {
+  const bool waits = PdlWaiting::all().next(stream, true), skip = pdl_skip_next() != 0;
+  pdl_skip_next() = 0;
+  return pdl_enabled() && !waits && !skip;
 }
 inline int& last_launch_error() {
   static thread_local int rc = 0;
@@ -180,8 +232,7 @@ inline void launch(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem,
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = (pdl_enabled() && !pdl_skip_next()) ? 1 : 0;
-  pdl_skip_next() = 0;
+  cfg.numAttrs = pdl_allowed(stream) ? 1 : 0;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
   if (e != cudaSuccess) last_launch_error() = (int)e;
 }
@@ -203,8 +254,7 @@ inline void launch_clusters(void (*kernel)(KArgs...), dim3 grid, dim3 block, siz
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = (pdl_enabled() && !pdl_skip_next()) ? 2 : 1;
-  pdl_skip_next() = 0;
+  cfg.numAttrs = pdl_allowed(stream) ? 2 : 1;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
   if (e != cudaSuccess) last_launch_error() = (int)e;
 }

@@ -417,7 +417,7 @@ int wpc_move_kept(void* k_pages, void* v_pages, int k_bytes, int v_bytes, float*
   else if (align % 4 == 0) go(move_kept_kernel<uint32_t>, (uint32_t*)k_pages, (uint32_t*)v_pages);
   else if (align % 2 == 0) go(move_kept_kernel<uint16_t>, (uint16_t*)k_pages, (uint16_t*)v_pages);
   else return WPC_ERR_UNSUPPORTED;
-  pdl_skip_next() = 1;      // (the kernel behind starts when the moves are done and visible)
+  PdlWaiting::all().add(stream);      // (the kernel behind starts when the moves are done and visible)
   return launch_status();
 }
 
