@@ -12,6 +12,8 @@ __global__ void embed_kernel(const int* __restrict__ tokens, const Tw* __restric
                              float* __restrict__ out, int H, int V) {
   pdl_trigger();
   pdl_wait();
+  tokens = after_wait(tokens);
+  table = after_wait(table);
   const int t = blockIdx.x;
   int id = tokens[t];
   if (id < 0 || id >= V) id = 0;                 // the host checks ids; never read outside
@@ -26,6 +28,7 @@ __global__ void rmsnorm_kernel(const float* __restrict__ x, const float* __restr
                                float eps, To* __restrict__ out, int H, const int* __restrict__ rows, int T) {
   pdl_trigger();
   pdl_wait();
+  x = after_wait(x);
   __shared__ float red[32];
   int src = rows ? rows[blockIdx.x] : (int)blockIdx.x;
   if (src < 0 || src >= T) src = 0;
@@ -74,6 +77,7 @@ __global__ void rmsnorm_vec_kernel(const float* __restrict__ x, const float* __r
     if (i < n4) g[k] = g4[i];
   }
   pdl_wait();
+  row = after_wait(row);
 #pragma unroll
   for (int k = 0; k < VPT; ++k) {
     const int i = threadIdx.x + k * blockDim.x;
@@ -100,6 +104,7 @@ template <typename T>
 __global__ void silu_mul_kernel(const T* __restrict__ gu, T* __restrict__ out, int I, int G, size_t n, int act) {
   pdl_trigger();
   pdl_wait();
+  gu = after_wait(gu);
   for (size_t i = (size_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (size_t)gridDim.x * blockDim.x) {
     const size_t t = i / I;
     const int c = (int)(i - t * I);
@@ -115,6 +120,7 @@ __global__ void silu_mul_vec_kernel(const __nv_bfloat16* __restrict__ gu, __nv_b
                                     int G, size_t n8, int act) {
   pdl_trigger();
   pdl_wait();
+  gu = after_wait(gu);
   for (size_t i = (size_t)blockIdx.x * blockDim.x + threadIdx.x; i < n8; i += (size_t)gridDim.x * blockDim.x) {
     const size_t e = i * 8;
     const size_t t = e / I;
@@ -140,6 +146,8 @@ template <typename T>
 __global__ void add_kernel(float* __restrict__ x, const T* __restrict__ y, size_t n) {
   pdl_trigger();
   pdl_wait();
+  x = after_wait(x);
+  y = after_wait(y);
   for (size_t i = (size_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (size_t)gridDim.x * blockDim.x)
     x[i] += to_float(y[i]);
 }
@@ -148,6 +156,7 @@ __global__ void gather_rows_kernel(const float* __restrict__ x, const int* __res
                                    float* __restrict__ out, int H, int T) {
   pdl_trigger();
   pdl_wait();
+  x = after_wait(x);
   int r = idx[blockIdx.x];
   if (r < 0 || r >= T) r = 0;
   const float* row = x + (size_t)r * H;
@@ -159,6 +168,7 @@ template <typename Ti, typename To>
 __global__ void convert_kernel(const Ti* __restrict__ in, To* __restrict__ out, size_t n) {
   pdl_trigger();
   pdl_wait();
+  in = after_wait(in);
   for (size_t i = (size_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (size_t)gridDim.x * blockDim.x)
     out[i] = from_float<To>(to_float(in[i]));
 }
@@ -193,6 +203,9 @@ __global__ void rope_inplace_kernel(T* __restrict__ x, int row_stride, int n_hea
                                     const float* __restrict__ cosv, const float* __restrict__ sinv, int interleaved) {
   pdl_trigger();
   pdl_wait();
+  x = after_wait(x);
+  cosv = after_wait(cosv);
+  sinv = after_wait(sinv);
   const int t = blockIdx.x, half = hd / 2;
   T* row = x + (size_t)t * row_stride;
   for (int i = threadIdx.x; i < n_heads * R; i += blockDim.x) {
@@ -214,6 +227,7 @@ __global__ void head_rmsnorm_kernel(T* __restrict__ x, int row_stride, int n_hea
                                     const float* __restrict__ gain, float eps, int T_rows) {
   pdl_trigger();
   pdl_wait();
+  x = after_wait(x);
   const int warp = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (warp >= T_rows * n_heads) return;
   const int t = warp / n_heads, h = warp - t * n_heads;
@@ -242,6 +256,9 @@ __global__ void qk_rope_kv_store_kernel(T* __restrict__ qkv, int row_stride, int
                                         int n_pages, int* __restrict__ status) {
   pdl_trigger();
   pdl_wait();
+  qkv = after_wait_global(qkv);
+  cosv = after_wait_global(cosv);
+  sinv = after_wait_global(sinv);
   const int t = blockIdx.x, half = hd / 2, lane = threadIdx.x & 31;
   const int head = blockIdx.y * ROPE_HEADS_PER_BLOCK + (threadIdx.x >> 5);
   if (head >= nh + 2 * nkv) return;

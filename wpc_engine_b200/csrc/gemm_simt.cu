@@ -18,6 +18,9 @@ gemm_simt_kernel(const Ta* __restrict__ A, int lda, const Tw* __restrict__ W, in
                  const float* __restrict__ bias, To* __restrict__ C, int ldc, int M, int N, int K) {
   pdl_trigger();
   pdl_wait();
+  A = after_wait_global(A);
+  W = after_wait_global(W);
+  C = after_wait_global(C);
   __shared__ float As[SG_BK][SG_BM + 4];
   __shared__ float Ws[SG_BK][SG_BN + 4];
   const int tid = threadIdx.x;
@@ -86,16 +89,18 @@ constexpr int GV_WARPS = 8;
 // k elements of every row of A in shared memory at a time (32 KiB at most)
 __host__ __device__ constexpr int gv_chunk(int mt) { return mt <= 8 ? 1024 : 512; }
 
+// (weights pass through once: through L2 only, 12.1 us at 1 x 896 x 4,864 against 12.4 with ordinary loads.  Not by
+// loads of constants, which are not tied to the dependency wait.)
 template <typename T> struct Vec4;
 template <> struct Vec4<float> {
   static __device__ __forceinline__ void load(const float* p, float (&v)[4]) {
-    const float4 t = __ldg((const float4*)p);
+    const float4 t = __ldcg((const float4*)p);
     v[0] = t.x; v[1] = t.y; v[2] = t.z; v[3] = t.w;
   }
 };
 template <> struct Vec4<__nv_bfloat16> {
   static __device__ __forceinline__ void load(const __nv_bfloat16* p, float (&v)[4]) {
-    const uint2 t = __ldg((const uint2*)p);
+    const uint2 t = __ldcg((const uint2*)p);
     const float2 a = __bfloat1622float2(*(const __nv_bfloat162*)&t.x), b = __bfloat1622float2(*(const __nv_bfloat162*)&t.y);
     v[0] = a.x; v[1] = a.y; v[2] = b.x; v[3] = b.y;
   }
@@ -121,6 +126,10 @@ gemv_simt_kernel(const Ta* __restrict__ A, int lda, const Tw* __restrict__ W, in
 #pragma unroll
   for (int f = 0; f < GV_FPW; ++f) wrow[f] = W + (size_t)min(f0 + f, N - 1) * ldw;     // rows past N repeat the last (not stored)
   pdl_wait();
+  A = after_wait_global(A);
+  C = after_wait_global(C);
+#pragma unroll
+  for (int f = 0; f < GV_FPW; ++f) wrow[f] = after_wait_global(wrow[f]);
   for (int k0 = 0; k0 < K; k0 += GV_CHUNK) {
     const int kc = min(GV_CHUNK, K - k0);
     __syncthreads();                                   // the chunk before has been used

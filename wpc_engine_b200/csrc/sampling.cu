@@ -43,6 +43,8 @@ sample_kernel(const float* __restrict__ logits, int V, const int* __restrict__ s
   const int lo = min(p_hi, p_lo + tid * chunk), hi = min(p_hi, lo + chunk);
   cluster_sync_all();                          // every rank runs: its shared memory may be written
   pdl_wait();
+  z = after_wait(z);
+  seq_state = after_wait(seq_state);
 
   // the first strictly greatest value: threads stride over the part (coalesced); among equal
   // values the lowest index wins, within a thread by order and between threads by comparison
