@@ -139,7 +139,7 @@ __global__ void attention_plain_combine_kernel(const float* __restrict__ part, T
   pdl_trigger();
   pdl_wait();
   const int t = blockIdx.x, h = blockIdx.y;
-  const float* prow = after_wait(part) + ((size_t)t * nh + h) * n_splits * (hd + 2);
+  const float* prow = after_wait_global(part) + ((size_t)t * nh + h) * n_splits * (hd + 2);
   float m = -INFINITY;
   for (int z = 0; z < n_splits; ++z) m = fmaxf(m, prow[(size_t)z * (hd + 2) + hd]);
   if (lse && threadIdx.x == 0) {
