@@ -143,3 +143,12 @@ def test_decode_behind_a_move_sees_what_was_moved(how):
         if want is None:
             want = got.clone()
         assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("lens,keep", [([51300], 51201), ([60000, 70000, 100], 52000)])
+def test_select_of_more_entries_than_shared_memory_lists(lens, keep):
+    sums, stored, table, _, _ = eviction_case(2, 1, lens, 8, hd=1)
+    after = [2500] * len(lens)
+    kept = ops.select_kept(sums, stored, table, ints(lens), ints(after), keep, 4, 10)
+    assert torch.equal(kept.cpu().long(), plain.select(sums, stored, table, lens, after, keep, 4, 10))
+    assert ops.device_status() == 0

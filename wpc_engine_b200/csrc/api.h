@@ -155,7 +155,9 @@ int wpc_weight_sums_mma(const void* q, int q_stride, const void* k_pages, const 
 // part (-1 behind a shorter sequence).  weight_sums, stored_positions: [layers][n_pages][nkv][64].
 int wpc_select_kept(const float* weight_sums, const int* stored_positions, const int* page_table, int table_width,
                     const int* lens, const int* next_positions, int layers, int B, int nkv, int n_pages,
-                    int keep, int sinks, int recent, int* kept, int* status, cudaStream_t stream);
+                    int keep, int sinks, int recent, int* kept, int* scratch, int* status, cudaStream_t stream);
+// ints of scratch memory that it needs for every (layer, sequence, KV head) (0: scratch may be null)
+long wpc_select_kept_scratch(int keep, int table_width);
 // k_bytes, v_bytes: bytes of an entry's key and value
 int wpc_move_kept(void* k_pages, void* v_pages, int k_bytes, int v_bytes, float* weight_sums, int* stored_positions,
                   const int* page_table, int table_width, const int* kept, int layers, int B, int nkv, int n_pages,

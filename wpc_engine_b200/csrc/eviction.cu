@@ -199,24 +199,26 @@ select_kept_kernel(const float* weight_sums, const int* stored_positions, size_t
 }
 
 // ---- any number of entries ----------------------------------------------------------------------------
-// The same with the keys made anew from the records each time, eight bits a digit.
+// The same with the keys made anew from the records each time, eight bits a digit.  The list of holes lies
+// in shared memory, or, where it has no room there, in `scratch`, [rows][keep].
 constexpr int SEL_THREADS = 1024;
 
 __global__ void __launch_bounds__(SEL_THREADS)
 select_kept_long_kernel(const float* weight_sums, const int* stored_positions, size_t layer_stride,
                         const int* __restrict__ page_table, int table_width, const int* __restrict__ lens,
                         const int* __restrict__ next_positions, int nkv, int n_pages, int keep, int sinks, int recent,
-                        int* kept, int* status) {
+                        int* kept, int* scratch, int* status) {
   pdl_trigger();
   pdl_wait();
   extern __shared__ int smem[];
-  int* const holes = smem;                              // [keep]
   __shared__ int hist[256];
   __shared__ int red[2][32];
   __shared__ uint32_t s_digit;
   __shared__ int s_want;
   const int g = blockIdx.x, b = blockIdx.y, layer = blockIdx.z, B = gridDim.y, tid = threadIdx.x;
-  int* const out = kept + (((size_t)layer * B + b) * nkv + g) * keep;
+  const size_t row = ((size_t)layer * B + b) * nkv + g;
+  int* const out = kept + row * keep;
+  int* const holes = scratch ? scratch + row * keep : smem;             // [keep]
   const int n = min(max(lens[b], 0), table_width * WPC_PAGE);
   if (n <= keep) {
     for (int i = tid; i < keep; i += SEL_THREADS) out[i] = i < n ? i : -1;
@@ -365,17 +367,28 @@ move_kept_kernel(V* k_pages, V* v_pages, int k_chunks, int v_chunks, float* weig
 
 using namespace wpc;
 
+// Places that the kernels keep in shared memory for every (layer, sequence, KV head); a table that holds
+// no more entries than are kept loses nothing.
+static int kept_places(int keep, int table_width) { return keep < (long)table_width * WPC_PAGE ? keep : 0; }
+constexpr int SEL_MAX_SHARED = 50 * 1024;
+
 extern "C" {
+
+long wpc_select_kept_scratch(int keep, int table_width) {
+  const int places = kept_places(keep, table_width);
+  return places > SEL_MAX_SHARED ? places : 0;
+}
 
 int wpc_select_kept(const float* weight_sums, const int* stored_positions, const int* page_table, int table_width,
                     const int* lens, const int* next_positions, int layers, int B, int nkv, int n_pages,
-                    int keep, int sinks, int recent, int* kept, int* status, cudaStream_t stream) {
+                    int keep, int sinks, int recent, int* kept, int* scratch, int* status, cudaStream_t stream) {
   if (layers <= 0 || B <= 0 || nkv <= 0) return 0;
   if (keep < 1 || sinks < 0 || recent < 0 || sinks > keep - recent || n_pages < 1 || table_width < 0) return WPC_ERR_BAD_ARGUMENT;
   if (layers > 65535 || B > 65535) return WPC_ERR_UNSUPPORTED;
-  const long n = (long)table_width * WPC_PAGE, most = 200 * 1024;
-  const int places = keep < n ? keep : 0;               // (a table that holds no more loses nothing)
-  if ((long)places * 4 > most) return WPC_ERR_TOO_LARGE;
+  const long n = (long)table_width * WPC_PAGE;
+  const int places = kept_places(keep, table_width);
+  const bool far = wpc_select_kept_scratch(keep, table_width) > 0;
+  if (far && !scratch) return WPC_ERR_BAD_ARGUMENT;
   const bool wide = (((uintptr_t)weight_sums | (uintptr_t)stored_positions) & 15) == 0;
   const dim3 grid(nkv, B, layers);
   const size_t layer_stride = (size_t)n_pages * nkv * WPC_PAGE;
@@ -394,9 +407,11 @@ int wpc_select_kept(const float* weight_sums, const int* stored_positions, const
   else if (wide && n <= 1024 * 32 && places <= 24 * 1024) WPC_SELECT(1024, 32);
   else {
     static int configured[MAX_DEVICES];
-    if (int rc = allow_smem(select_kept_long_kernel, places * 4, configured)) return rc;
-    wpc::launch(select_kept_long_kernel, grid, SEL_THREADS, places * 4, stream, weight_sums, stored_positions, layer_stride,
-                page_table, table_width, lens, next_positions, nkv, n_pages, keep, sinks, recent, kept, status);
+    const int smem = far ? 0 : places * 4;
+    if (int rc = allow_smem(select_kept_long_kernel, smem, configured)) return rc;
+    wpc::launch(select_kept_long_kernel, grid, SEL_THREADS, smem, stream, weight_sums, stored_positions, layer_stride,
+                page_table, table_width, lens, next_positions, nkv, n_pages, keep, sinks, recent, kept,
+                far ? scratch : nullptr, status);
   }
 #undef WPC_SELECT
   return launch_status();

@@ -307,11 +307,15 @@ at::Tensor select_kept(const Args& a) {
   if (!is(next, at::kInt, r.B, r.device)) refuse("next_positions must be contiguous int32 [B]");
   at::Tensor kept = ws.dim() == 3 ? empty({r.B, r.nkv, keep}, at::kInt, r.device)
                                   : empty({r.layers, r.B, r.nkv, keep}, at::kInt, r.device);
-  if (kept.numel())
-    launched("select_kept", wpc_select_kept(r.sums, r.stored, r.table, r.width, lens.data_ptr<int>(), next.data_ptr<int>(),
-                                            r.layers, r.B, r.nkv, r.n_pages, keep, sinks, recent, kept.data_ptr<int>(),
-                                            (int*)a.tensor(8, "status").data_ptr(),
-                                            c10::cuda::getCurrentCUDAStream(r.device).stream()));
+  if (!kept.numel()) return kept;
+  at::Tensor scratch;
+  if (const long places = wpc_select_kept_scratch(keep, r.width))
+    scratch = empty({(long)r.layers * r.B * r.nkv * places}, at::kInt, r.device);
+  launched("select_kept", wpc_select_kept(r.sums, r.stored, r.table, r.width, lens.data_ptr<int>(), next.data_ptr<int>(),
+                                          r.layers, r.B, r.nkv, r.n_pages, keep, sinks, recent, kept.data_ptr<int>(),
+                                          scratch.defined() ? scratch.data_ptr<int>() : nullptr,
+                                          (int*)a.tensor(8, "status").data_ptr(),
+                                          c10::cuda::getCurrentCUDAStream(r.device).stream()));
   return kept;
 }
 
