@@ -152,3 +152,36 @@ def test_select_of_more_entries_than_shared_memory_lists(lens, keep):
     kept = ops.select_kept(sums, stored, table, ints(lens), ints(after), keep, 4, 10)
     assert torch.equal(kept.cpu().long(), plain.select(sums, stored, table, lens, after, keep, 4, 10))
     assert ops.device_status() == 0
+
+
+def test_a_cut_of_many_sequences():
+    """More pairs of a sequence and a KV head than a grid has rows."""
+    B, nkv, keep = 33000, 2, 3
+    sums = torch.rand((1, B, nkv, PAGE), generator=torch.Generator().manual_seed(1)).to(DEV)
+    stored = torch.arange(PAGE, dtype=torch.int32, device=DEV).expand(1, B, nkv, PAGE).contiguous()
+    table = torch.randperm(B, generator=torch.Generator().manual_seed(2)).int().view(B, 1).to(DEV)
+    k, v = (rnd((1, B, nkv, PAGE, 2), torch.bfloat16, seed) for seed in (3, 4))
+    lens, after = torch.full((B,), 5, dtype=torch.int32, device=DEV), torch.full((B,), 5, dtype=torch.int32, device=DEV)
+    kept = ops.select_kept(sums, stored, table, lens, after, keep, 0, 1)
+    pages = table[:, 0].long()
+    want = [t.clone() for t in (k, v, sums, stored)]
+    # (the last position, entry 4, always stays)
+    score = sums[0, pages, :, :5].clone()
+    score[..., 4] = 9.0
+    best = score.argsort(dim=-1, descending=True)[..., :keep].sort(dim=-1).values          # [B, nkv, keep]
+    place = torch.arange(keep, device=DEV).expand(B, nkv, keep).clone()
+    inside = torch.zeros((B, nkv, 5), dtype=torch.bool, device=DEV).scatter_(2, best, True)
+    movers = best.masked_fill(best < keep, 99).sort(dim=-1).values
+    holes = (~inside[..., :keep]).cumsum(-1) - 1
+    expect = torch.where(inside[..., :keep], place, movers.gather(2, holes.clamp(min=0)))
+    assert torch.equal(kept[0].long(), expect)
+    at = expect
+    for t in want:
+        rows = t[0, pages]
+        index = at if rows.dim() == 3 else at[..., None].expand(-1, -1, -1, rows.shape[-1])
+        new = rows.clone()
+        new[:, :, :keep] = rows.gather(2, index)
+        t[0, pages] = new
+    ops.move_kept_(k, v, sums, stored, table, kept)
+    assert all(torch.equal(a, b) for a, b in zip((k, v, sums, stored), want))
+    assert ops.device_status() == 0

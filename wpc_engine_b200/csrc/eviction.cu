@@ -311,8 +311,8 @@ move_kept_kernel(V* k_pages, V* v_pages, int k_chunks, int v_chunks, float* weig
   __shared__ int s_n;
   if (threadIdx.x == 0) s_n = 0;
   pdl_wait();
-  const int g = blockIdx.y % nkv, b = blockIdx.y / nkv, layer = blockIdx.z, tid = threadIdx.x, lane = tid & 31;
-  const int i = blockIdx.x * MOVE_PLACES + tid;
+  const int g = blockIdx.x % nkv, b = blockIdx.x / nkv, layer = blockIdx.z, tid = threadIdx.x, lane = tid & 31;
+  const int i = blockIdx.y * MOVE_PLACES + tid;
   const int* table = page_table + (size_t)b * table_width;
   const int src = i < keep ? kept[(((size_t)layer * B + b) * nkv + g) * keep + i] : -1;
   long from = 0, to = 0;
@@ -421,8 +421,9 @@ int wpc_move_kept(void* k_pages, void* v_pages, int k_bytes, int v_bytes, float*
                   const int* page_table, int table_width, const int* kept, int layers, int B, int nkv, int n_pages,
                   int keep, int* status, cudaStream_t stream) {
   if (layers <= 0 || B <= 0 || nkv <= 0 || keep <= 0) return 0;
-  if (layers > 65535 || (long)B * nkv > 65535) return WPC_ERR_TOO_LARGE;
-  const dim3 grid((keep + MOVE_PLACES - 1) / MOVE_PLACES, (unsigned)(B * nkv), (unsigned)layers);
+  const int chunks = (keep - 1) / MOVE_PLACES + 1;
+  if (layers > 65535 || (long)B * nkv > 0x7fffffffL || chunks > 65535) return WPC_ERR_TOO_LARGE;
+  const dim3 grid((unsigned)(B * nkv), (unsigned)chunks, (unsigned)layers);
   const uintptr_t align = (uintptr_t)k_pages | (uintptr_t)v_pages | (uintptr_t)k_bytes | (uintptr_t)v_bytes;
   auto go = [&](auto kernel, auto* k, auto* v) {
     wpc::launch(kernel, grid, MOVE_THREADS, 0, stream, k, v, k_bytes / (int)sizeof(*k), v_bytes / (int)sizeof(*v), weight_sums,
