@@ -189,8 +189,15 @@ class Engine:
         step, which waits for the device, and raise `KernelError` if a kernel of the step gave
         up.  A step that raises, for whatever reason, leaves the sequences as they were: the
         pages that it had taken go back.  (With eviction a step that a kernel gave up in may have added
-        to the sums of entries stored before it.)"""
+        to the sums of entries stored before it.)
+
+        With eviction, sequences that hold too many entries afterwards are cut down to what is kept.  If
+        that cannot be done (no memory for the choice), the step still counts and its logits are
+        returned: the sequence's next step begins with the cut, and raises if it fails again."""
         self._check(entries)
+        left_over = self.cache.over([e.slot for e in entries])
+        if left_over:
+            self._evict(left_over)
         reserved = []
         try:
             starts = []
@@ -209,7 +216,10 @@ class Engine:
         self.steps_run += 1
         over = self.cache.over([e.slot for e in entries])
         if over:
-            self._evict(over)
+            try:
+                self._evict(over)
+            except (ops.KernelError, torch.OutOfMemoryError):
+                pass                       # (the tokens are stored: tried again before these sequences take more pages)
         return logits
 
     def _evict(self, slots: Sequence[int]) -> None:
@@ -217,6 +227,7 @@ class Engine:
         pages go back at once, since what is queued later runs later)."""
         e = self.cache.eviction
         n = len(slots)
+        chosen = []                        # for every group before the first is moved: a choice may fail, moves take no memory
         for i in self.cache.evicting_groups():
             group = self.cache.groups[i]
             width = max(len(group.tables[s]) for s in slots)
@@ -230,6 +241,8 @@ class Engine:
             table = meta[2 * n:].view(n, width)
             kept = ops.select_kept(group.weight_sums, group.stored_positions, table, meta[: n], meta[n: 2 * n],
                                    e.keep, e.sinks, e.recent)
+            chosen.append((group, table, kept))
+        for group, table, kept in chosen:
             ops.move_kept_(group.k, group.v, group.weight_sums, group.stored_positions, table, kept)
         for s in slots:
             self.cache.cut(s)
