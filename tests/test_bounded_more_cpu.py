@@ -83,3 +83,43 @@ def test_no_group_is_moved_if_the_choice_of_another_fails(tmp_path, bounded_cpu_
         eng._evict([slot])
     assert len(calls) == 2 and eng.cache.stored[slot] == 100
     assert all(torch.equal(k, g.k) for k, g in zip(before, eng.cache.groups))
+
+
+@pytest.mark.parametrize("flags,pages", [
+    (["--cache-keep", "1024", "--max-step-tokens", "512"], 1 * 25),                       # 1,024 + 64 + 512 entries
+    (["--cache-keep", "1024", "--max-step-tokens", "512", "--max-batch", "8"], 1 * 25),   # (one prompt, one sequence)
+    (["--max-step-tokens", "512"], 1563)])
+def test_the_command_line_bounds_the_cache_by_what_is_kept(tmp_path, monkeypatch, flags, pages):
+    """100,000 positions of a model whose positions go that far: the cache is as large as what is kept."""
+    from wpc_engine_b200 import cli
+    cfg = wpc.Qwen2Config.from_dict(dict(TINY_A, max_position_embeddings=1 << 20))
+    wpc.write_random_model(str(tmp_path), cfg, 1, torch.float32)
+    asked = {}
+
+    class Seen(Exception):
+        pass
+
+    def from_folder(folder, **kw):
+        asked.update(kw)
+        raise Seen
+    monkeypatch.setattr(wpc.Engine, "from_folder", from_folder)
+    with pytest.raises(Seen):
+        cli.main(["--model", str(tmp_path), "--dtype", "fp32", "--prompt-ids", "1,2,3,4", "--max-tokens", "99996", *flags])
+    from wpc_engine_b200.cache import SequenceCache
+    from wpc_engine_b200.parts.base import KVSpec
+    cache = SequenceCache([KVSpec(2, 16)], asked["max_tokens"], torch.float32, "cpu", asked.get("max_sequences"),
+                          asked["max_step_tokens"], asked["eviction"])
+    assert cache.groups[0].n_pages == pages
+    assert cache.fits([100000])
+
+
+def test_the_command_line_has_room_for_every_sequence_of_a_batch(tmp_path, monkeypatch):
+    from wpc_engine_b200 import cli
+    cfg = wpc.Qwen2Config.from_dict(TINY_A)
+    wpc.write_random_model(str(tmp_path), cfg, 1, torch.float32)
+    asked = []
+    monkeypatch.setattr(wpc.Engine, "from_folder", lambda folder, **kw: asked.append(kw["max_sequences"]) or 1 / 0)
+    for flags, n in (([], 3), (["--max-batch", "2"], 2), (["--max-batch", "9"], 3)):
+        with pytest.raises(ZeroDivisionError):
+            cli.main(["--model", str(tmp_path), "--prompt-ids", "1,2;3;4", "--max-tokens", "4", *flags])
+        assert asked[-1] == n

@@ -48,7 +48,8 @@ def build_parser() -> argparse.ArgumentParser:
     ap.add_argument("--max-step-tokens", type=int, default=None, help="feed prompts in chunks of that many tokens")
     ap.add_argument("--cache-keep", type=int, default=None,
                     help="entries that a sequence keeps in layers without a window: the first, the last, and those with "
-                         "the most attention weight (default: all)")
+                         "the most attention weight (default: all); with --max-step-tokens the cache holds no more than that, "
+                         "a page or two and a step for each sequence")
     ap.add_argument("--cache-recent", type=int, default=None,
                     help="last positions that --cache-keep always holds (default: a quarter of it)")
     ap.add_argument("--cache-sinks", type=int, default=4, help="first positions that --cache-keep always holds")
@@ -119,8 +120,9 @@ def main(argv=None) -> int:
     need = sum((len(p) + args.max_tokens + PAGE - 1) // PAGE * PAGE for p in prompts)
     if args.max_batch:
         need = max((len(p) + args.max_tokens + PAGE - 1) // PAGE * PAGE for p in prompts) * args.max_batch
+    # (as many sequences as can be alive at once: what bounds a sequence's pages then bounds the cache)
     engine = Engine.from_folder(args.model, dtype=dtype, device="cuda", max_tokens=args.cache_tokens or need,
-                                max_step_tokens=args.max_step_tokens, eviction=eviction)
+                                max_sequences=min(len(prompts), args.max_batch or len(prompts)), max_step_tokens=args.max_step_tokens, eviction=eviction)
     c = engine.config
     print(f"config: hidden={c.hidden_size} layers={c.num_hidden_layers} heads={c.num_attention_heads} "
           f"kv_heads={c.num_key_value_heads} vocab={c.vocab_size}", file=sys.stderr)

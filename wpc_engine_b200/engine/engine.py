@@ -78,9 +78,11 @@ class Engine:
     error word after it has run (which waits for the device) and raises `KernelError` if a
     kernel gave up; callers that keep the device busy pass `check=False` to `step` and read the
     word with their results (`generate` does).  eviction: what the layers without a window keep of a
-    sequence that outgrows it (`CacheEviction`; None: everything).  With `max_step_tokens` the cache is
-    sized by it; without, a step that brings a whole prompt needs pages for all of it until it
-    has run.
+    sequence that outgrows it (`CacheEviction`; None: everything).  With `max_step_tokens` and
+    `max_sequences` the cache is sized by it: keep + slack + a step's tokens for each sequence, whatever
+    max_tokens says beyond that (without max_sequences there may be as many sequences as max_tokens has
+    pages).  Without max_step_tokens a step that brings a whole prompt needs pages for all of it until
+    it has run.
 
     The limits of a step come from the model: `model.vocab_size` and `model.max_positions`."""
 
