@@ -123,3 +123,26 @@ def test_the_command_line_has_room_for_every_sequence_of_a_batch(tmp_path, monke
         with pytest.raises(ZeroDivisionError):
             cli.main(["--model", str(tmp_path), "--prompt-ids", "1,2;3;4", "--max-tokens", "4", *flags])
         assert asked[-1] == n
+
+
+def test_a_captured_step_is_planned_for_what_is_kept(tmp_path, bounded_cpu_ops):
+    """A table that is wide for a windowed layer's sake does not make the evicting layers' steps larger."""
+    e = CacheEviction(keep=40, recent=10, sinks=3, slack=8)
+    eng = engine_of(tmp_path, dict(TINY_C, max_position_embeddings=4096), max_tokens=4096, max_sequences=2, eviction=e)
+    assert [eng._most_stored(w) for w in (1, 2, 64)] == [49, 49, 49]
+    eng = engine_of(tmp_path, TINY_C, max_tokens=4096, max_sequences=2, eviction=CacheEviction(keep=100, recent=10))
+    assert [eng._most_stored(w) for w in (1, 2, 64)] == [64, 128, 165]
+    # and never for less than a step stores
+    slot = eng.open_sequence()
+    most = []
+    plan = wpc.engine.engine.plan_step
+    wpc.engine.engine.plan_step = lambda *a, **kw: most.append(plan(*a, **kw)) or most[-1]
+    try:
+        eng.step([SequenceStep(slot, ids(150))])
+        for i in range(150):
+            eng.step([SequenceStep(slot, [i])])
+    finally:
+        wpc.engine.engine.plan_step = plan
+    widths = {p.layout.table_width for p in most[1:]}
+    assert len(widths) > 1 and all(p.max_stored_len <= eng._most_stored(p.layout.table_width) for p in most[1:])
+    assert max(p.max_stored_len for p in most[1:]) == 165

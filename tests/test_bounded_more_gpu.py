@@ -6,6 +6,8 @@ import pytest
 import torch
 
 import bounded_plain as plain
+import wpc_engine_b200 as wpc
+from conftest import TINY_C
 from test_bounded_gpu import DEV, PAGE, Step, eviction_case, fast_want, ints, rnd
 from wpc_engine_b200 import ops
 
@@ -185,3 +187,29 @@ def test_a_cut_of_many_sequences():
     ops.move_kept_(k, v, sums, stored, table, kept)
     assert all(torch.equal(a, b) for a, b in zip((k, v, sums, stored), want))
     assert ops.device_status() == 0
+
+
+def test_captured_steps_of_evicting_layers_are_planned_for_what_is_kept(tmp_path, monkeypatch):
+    """Windowed layers widen the page table with the position; the evicting layer's attention is captured
+    for keep + slack + 1 entries all the same, and gives what uncaptured steps give (in 32 bits, whose split
+    is the same for all such lengths)."""
+    raw = dict(TINY_C, max_position_embeddings=4096)
+    wpc.write_random_model(str(tmp_path), wpc.Qwen2Config.from_dict(raw), 3, torch.float32)
+    e = wpc.CacheEviction(keep=60, recent=20, sinks=2, slack=16)
+    captured, plain_attention = [], ops.attention
+
+    def attention(*args, **kw):
+        if torch.cuda.is_current_stream_capturing() and "weight_sums" in kw:
+            captured.append(args[14])
+        return plain_attention(*args, **kw)
+    monkeypatch.setattr(ops, "attention", attention)
+    prompt = torch.randint(0, 290, (900,), generator=torch.Generator().manual_seed(1)).tolist()
+    rows = []
+    for graphs in (True, False):
+        eng = wpc.Engine.from_folder(str(tmp_path), dtype="float32", max_tokens=2048, max_sequences=1, use_graphs=graphs, eviction=e)
+        s = eng.open_sequence()
+        got = [eng.step([wpc.SequenceStep(s, prompt, want=[899])])]
+        got += [eng.step([wpc.SequenceStep(s, [i], want=[0])]) for i in range(200)]
+        rows.append((torch.cat(got), *eng.stored_positions(s)))
+    assert captured and set(captured) == {77}
+    assert all(torch.equal(a, b) for a, b in zip(*rows))

@@ -292,6 +292,12 @@ class Engine:
             logits = self.model.forward(ctx, self.cache)
         return logits
 
+    def _most_stored(self, table_width: int) -> int:
+        """The most entries that a group which evicts holds of a sequence after a single-token step: the
+        table is as wide as the widest group needs, which may be one that keeps every position."""
+        e, most = self.cache.eviction, table_width * PAGE
+        return most if e is None else min(most, e.keep + e.slack + 1)
+
     def _graph_step(self, plan, host: torch.Tensor, device_tokens: Optional[torch.Tensor] = None):
         """Single-token steps of a shape seen before are replayed from a CUDA graph.  The first
         step of a shape runs directly (returns ran=False); the second is captured, which runs
@@ -305,7 +311,7 @@ class Engine:
         if entry == "seen":
             meta = torch.zeros(lay.total, dtype=torch.int32, device=self.device)
             ctx = context_from(meta, lay, self.dtype, 1, lay.table_width * PAGE, True,
-                               max_stored_len=lay.table_width * PAGE)
+                               max_stored_len=self._most_stored(lay.table_width))
             graph = torch.cuda.CUDAGraph()
             before = ops.launch_count
             with torch.cuda.graph(graph):
