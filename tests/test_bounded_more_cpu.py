@@ -146,3 +146,20 @@ def test_a_captured_step_is_planned_for_what_is_kept(tmp_path, bounded_cpu_ops):
     widths = {p.layout.table_width for p in most[1:]}
     assert len(widths) > 1 and all(p.max_stored_len <= eng._most_stored(p.layout.table_width) for p in most[1:])
     assert max(p.max_stored_len for p in most[1:]) == 165
+
+
+def test_a_built_extension_module_loads_without_a_cuda_toolkit(tmp_path, monkeypatch):
+    from wpc_engine_b200.csrc import build
+
+    def no_nvcc():
+        raise build.BuildError("nvcc was not found")
+    monkeypatch.setattr(build, "find_nvcc", no_nvcc)
+    monkeypatch.setattr(build, "library_path", lambda verbose=True: str(tmp_path / build.LIB_NAME))
+    with pytest.raises(build.BuildError, match="nvcc"):
+        build.host_module_path(False)
+    (tmp_path / build.HOST_NAME).write_bytes(b"")
+    (tmp_path / "host_stamp").write_text(build._host_stamp())
+    assert build.host_module_path(False) == str(tmp_path / build.HOST_NAME)
+    (tmp_path / "host_stamp").write_text("another")
+    with pytest.raises(build.BuildError, match="nvcc"):
+        build.host_module_path(False)

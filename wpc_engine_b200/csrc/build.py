@@ -127,31 +127,41 @@ def library_path(verbose: bool = True) -> str:
     return lib
 
 
+def _host_flags() -> List[str]:
+    import torch
+    return ["-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
+            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
+
+
+def _host_stamp() -> str:
+    """What the extension module is made from and for."""
+    import torch
+    return "\n".join([_digest(["host.cpp", "api.h"]), torch.__version__, sys.version] + _host_flags())
+
+
 def host_module_path(verbose: bool = True) -> str:
     """The path of an up-to-date extension module, linked against the kernel library and torch."""
-    import sysconfig
-
-    import torch
     lib = library_path(verbose)
     out_dir = os.path.dirname(lib)
     path, stamp_path = os.path.join(out_dir, HOST_NAME), os.path.join(out_dir, "host_stamp")
-    root = os.path.dirname(torch.__file__)
-    cuda = os.path.dirname(os.path.dirname(os.path.realpath(find_nvcc())))
-    flags = ["-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
-             f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
-    want = "\n".join([_digest(["host.cpp", "api.h"]), torch.__version__, sys.version] + flags)
+    want = _host_stamp()
     try:
         with open(stamp_path) as f:
             if f.read() == want and os.path.exists(path):
                 return path
     except OSError:
         pass
+    import sysconfig
+
+    import torch
+    root = os.path.dirname(torch.__file__)
+    cuda = os.path.dirname(os.path.dirname(os.path.realpath(find_nvcc())))      # (a module that is built needs no toolkit)
     t0 = time.time()
     if verbose:
         _say("compiling host.cpp")
     tmp = path + f".tmp{os.getpid()}"
     libs = os.path.join(root, "lib")
-    cmd = ["g++"] + flags + [os.path.join(HERE, "host.cpp"), "-o", tmp, "-I", HERE, "-I", os.path.join(root, "include"),
+    cmd = ["g++"] + _host_flags() + [os.path.join(HERE, "host.cpp"), "-o", tmp, "-I", HERE, "-I", os.path.join(root, "include"),
            "-I", os.path.join(root, "include", "torch", "csrc", "api", "include"), "-I", os.path.join(cuda, "include"),
            "-I", sysconfig.get_paths()["include"], "-L", out_dir, f"-l:{LIB_NAME}", "-L", libs, "-lc10", "-lc10_cuda",
            "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python", "-L", os.path.join(cuda, "lib64"), "-lcudart",
