@@ -163,3 +163,42 @@ def test_a_built_extension_module_loads_without_a_cuda_toolkit(tmp_path, monkeyp
     (tmp_path / "host_stamp").write_text("another")
     with pytest.raises(build.BuildError, match="nvcc"):
         build.host_module_path(False)
+
+
+def test_plans_follow_the_switches_and_the_device(monkeypatch):
+    """A plan that was made is not used again for another device or after a switch was set."""
+    fits = {"now": lambda hd, c, alone: 8 if c <= 8 else 4}
+    monkeypatch.setattr(ops, "decode_cluster_capacity", lambda *a: fits["now"](*a))
+    args = (1, 4, 28, 128, 66, None, None, 1, 148)
+    ops._bounded_decode_plan.cache_clear()
+    try:
+        with_clusters = ops._bounded_decode_plan(*args, ops._plan_switches(0))
+        assert with_clusters[0] > 0
+        fits["now"] = lambda hd, c, alone: 0                    # another chip, that takes no clusters
+        assert ops._bounded_decode_plan(*args, ops._plan_switches(1))[0] == 0
+        assert ops._bounded_decode_plan(*args, ops._plan_switches(0)) == with_clusters
+        for name, value in (("CLUSTER_DECODE", False), ("CLUSTER_DECODE_MAX_OUT", 16), ("CLUSTER_EXCHANGE_US", 1000.0)):
+            with monkeypatch.context() as m:
+                fits["now"] = lambda hd, c, alone: 8 if c <= 8 else 4
+                m.setattr(ops, name, value)
+                assert ops._bounded_decode_plan(*args, ops._plan_switches(0))[0] == 0, name
+    finally:
+        ops._bounded_decode_plan.cache_clear()
+
+
+def test_cluster_capacities_are_asked_for_every_device(monkeypatch):
+    class Library:
+        asked = []
+
+        def wpc_attention_decode_cluster_capacity(self, hd, cluster, alone):
+            self.asked.append(device["now"])
+            return 10 + device["now"]
+    device = {"now": 0}
+    monkeypatch.setattr(ops, "library", Library)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: device["now"])
+    monkeypatch.setattr(ops, "_decode_cluster_capacity", {})
+    assert ops.decode_cluster_capacity(128, 4, True) == 10
+    device["now"] = 1
+    assert ops.decode_cluster_capacity(128, 4, True) == 11
+    device["now"] = 0
+    assert ops.decode_cluster_capacity(128, 4, True) == 10 and Library.asked == [0, 1]

@@ -745,14 +745,21 @@ def attention(q: torch.Tensor, n_heads: int, n_kv_heads: int, head_dim: int, k_p
 
 
 @functools.lru_cache(maxsize=4096)
-def _bounded_decode_plan(n_seqs, n_kv_heads, n_heads, head_dim, blocks, splits, cluster, groups, n_sms):
-    """(cluster, groups, n_ctas) of a decode step in which a query sees `blocks` pages."""
+def _bounded_decode_plan(n_seqs, n_kv_heads, n_heads, head_dim, blocks, splits, cluster, groups, n_sms, switches=None):
+    """(cluster, groups, n_ctas) of a decode step in which a query sees `blocks` pages.  n_sms and `switches` are
+    there for the cache's sake: what else a plan depends on (`_plan_switches`)."""
     if n_kv_heads < 1 or n_heads % n_kv_heads:
         raise KernelError(f"n_heads must be a multiple of n_kv_heads, got {n_heads} and {n_kv_heads}")
     ctx = blocks * PAGE
     if cluster is None:
         cluster, groups = (0, 1) if splits else plan_decode_cluster(n_seqs, n_kv_heads, n_heads, head_dim, ctx, None)
     return cluster, groups, 0 if cluster else plan_decode_ctas(n_seqs, n_kv_heads, ctx, None, splits)
+
+
+def _plan_switches(device):
+    """The device, whose GPCs say which clusters fit, and the module's switches that plans go by."""
+    return (device, CLUSTER_DECODE, CLUSTER_DECODE_MAX_OUT, CLUSTER_PAGE_ALONE_US, CLUSTER_PAGE_SHARED_US, CLUSTER_SHARED_START_US,
+            CLUSTER_EXCHANGE_US, GROUP_COMBINE_US, GROUP_EACH_US)
 
 
 def _bounded_attention(q, n_heads, n_kv_heads, head_dim, k_pages, v_pages, page_table, cu_seqlens, ctx_lens, seq_of_token,
@@ -770,7 +777,7 @@ def _bounded_attention(q, n_heads, n_kv_heads, head_dim, k_pages, v_pages, page_
         if window:
             blocks = min(blocks, -(-window // PAGE) + 1 + -(-sinks // PAGE))
         cluster, groups, n_ctas = _bounded_decode_plan(ctx_lens.numel(), n_kv_heads, n_heads, head_dim, blocks, splits, cluster,
-                                                       groups, n_sms)
+                                                       groups, n_sms, _plan_switches(device))
     out = (_host or host()).attention(
         q, n_heads, n_kv_heads, head_dim, k_pages, v_pages, page_table, cu_seqlens, ctx_lens, seq_of_token, positions, scale,
         window or 0, max_new_tokens, max_ctx_len, mma_only, sinks, weight_sums, stored_positions, token_positions,
@@ -877,7 +884,7 @@ _decode_cluster_capacity: dict = {}
 def decode_cluster_capacity(head_dim: int, cluster: int, alone: bool) -> int:
     """Clusters of `cluster` CTAs of the cluster decode kernel that this device runs at once
     (a cluster lives inside one GPC, and chips differ in the SMs that their GPCs have)."""
-    key = (head_dim, cluster, alone)
+    key = (torch.cuda.current_device(), head_dim, cluster, alone)
     if key not in _decode_cluster_capacity:
         _decode_cluster_capacity[key] = max(0, int(library().wpc_attention_decode_cluster_capacity(
             head_dim, cluster, int(alone))))
