@@ -213,3 +213,20 @@ def test_captured_steps_of_evicting_layers_are_planned_for_what_is_kept(tmp_path
         rows.append((torch.cat(got), *eng.stored_positions(s)))
     assert captured and set(captured) == {77}
     assert all(torch.equal(a, b) for a, b in zip(*rows))
+
+
+def test_numbers_that_are_none_are_refused():
+    s = Step(torch.bfloat16, 14, 2, 64, [300, 70], [3, 1], 100, 4, seed=1)
+    args = [s.q, *s.heads, s.k, s.v, s.table, s.cu, s.ctx, s.seq, s.pos, s.scale, 100, 3, 300]
+    for at, name, bads in ((1, "n_heads", ("three", [3], None, 2.5, 1 << 70)), (11, "scale", ("three", [3], None)),
+                           (12, "window", (2.5, 1 << 70)), (13, "max_new_tokens", ("three", [3], None, 2.5, 1 << 70, 1 << 40))):
+        for bad in bads:
+            with pytest.raises(ops.KernelError, match=name):
+                ops.attention(*args[:at], bad, *args[at + 1:], sinks=4)
+    sums, stored, table, _, _ = eviction_case(1, 1, [200], 1)
+    for at, name in ((0, "keep"), (1, "sinks"), (2, "recent")):
+        numbers = [64, 4, 8]
+        numbers[at] += 0.5
+        with pytest.raises(ops.KernelError, match=name):
+            ops.select_kept(sums, stored, table, ints([200]), ints([200]), *numbers)
+    assert ops.device_status() == 0

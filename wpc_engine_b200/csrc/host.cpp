@@ -13,6 +13,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <algorithm>
+#include <climits>
 #include <map>
 #include <string>
 #include <utility>
@@ -39,6 +40,11 @@ void launched(const char* name, int rc) {
   refuse(std::string(name) + ": " + (what ? std::string(what) : "CUDA error " + std::to_string(rc)));
 }
 
+int as_int(long v, const char* name) {
+  if (v < 0 || v > 0x7fffffff) refuse(std::string(name) + " is out of range");
+  return (int)v;
+}
+
 struct Args {
   PyObject* const* a;
   const at::Tensor& tensor(int i, const char* name) const {
@@ -46,15 +52,26 @@ struct Args {
     return THPVariable_Unpack(a[i]);
   }
   bool none(int i) const { return a[i] == Py_None; }
-  long number(int i) const {
+  // (a number that is none raises the library's error like any other argument that is not taken)
+  long number(int i, const char* name) const {
     const long v = PyLong_AsLong(a[i]);
-    if (v == -1 && PyErr_Occurred()) throw Refused();
+    if (v == -1 && PyErr_Occurred()) not_taken(name, "a whole number");
     return v;
   }
-  double real(int i) const {
+  double real(int i, const char* name) const {
     const double v = PyFloat_AsDouble(a[i]);
-    if (v == -1.0 && PyErr_Occurred()) throw Refused();
+    if (v == -1.0 && PyErr_Occurred()) not_taken(name, "a number");
     return v;
+  }
+  int integer(int i, const char* name, long most = LONG_MAX) const {
+    return as_int(std::min(number(i, name), most), name);
+  }
+
+ private:
+  [[noreturn]] static void not_taken(const char* name, const char* what) {
+    if (!PyErr_ExceptionMatches(PyExc_TypeError) && !PyErr_ExceptionMatches(PyExc_OverflowError)) throw Refused();
+    PyErr_Clear();
+    refuse(std::string(name) + " must be " + what);
   }
 };
 
@@ -73,10 +90,6 @@ int current_device_of(const at::Tensor& t, const char* name) {
   return device;
 }
 uintptr_t address(const at::Tensor& t) { return (uintptr_t)t.data_ptr(); }
-int as_int(long v, const char* name) {
-  if (v < 0 || v > 0x7fffffff) refuse(std::string(name) + " is out of range");
-  return (int)v;
-}
 
 at::Tensor empty(c10::IntArrayRef size, at::ScalarType type, int device) {
   return at::detail::empty_cuda(size, type, c10::Device(c10::kCUDA, (c10::DeviceIndex)device), std::nullopt);
@@ -129,12 +142,12 @@ at::Tensor attention(const Args& a) {
   const at::Tensor &q = a.tensor(0, "q"), &k = a.tensor(4, "k_pages"), &v = a.tensor(5, "v_pages"),
                    &table = a.tensor(6, "page_table"), &cu = a.tensor(7, "cu_seqlens"), &ctx = a.tensor(8, "ctx_lens"),
                    &seq = a.tensor(9, "seq_of_token"), &pos = a.tensor(10, "positions");
-  const int nh = as_int(a.number(1), "n_heads"), nkv = as_int(a.number(2), "n_kv_heads"), hd = as_int(a.number(3), "head_dim");
-  const float scale = (float)a.real(11);
-  const int window = as_int(std::min(a.number(12), 1L << 30), "window");
-  const int max_new = as_int(a.number(13), "max_new_tokens"), max_ctx = as_int(a.number(14), "max_ctx_len");
-  const bool mma_only = a.number(15) != 0, sums = !a.none(17);
-  const int sinks = as_int(std::min(a.number(16), 1L << 30), "sinks");
+  const int nh = a.integer(1, "n_heads"), nkv = a.integer(2, "n_kv_heads"), hd = a.integer(3, "head_dim");
+  const float scale = (float)a.real(11, "scale");
+  const int window = a.integer(12, "window", 1L << 30);
+  const int max_new = a.integer(13, "max_new_tokens"), max_ctx = a.integer(14, "max_ctx_len");
+  const bool mma_only = a.number(15, "mma_only") != 0, sums = !a.none(17);
+  const int sinks = a.integer(16, "sinks", 1L << 30);
   const int device = current_device_of(q, "q");
   const at::ScalarType type = q.scalar_type();
   if (type != at::kBFloat16 && type != at::kFloat) refuse("unsupported element type");
@@ -173,7 +186,7 @@ at::Tensor attention(const Args& a) {
   if (T == 0) return out;
   if (B < 1) refuse("q has tokens, but there are no sequences");
   const cudaStream_t stream = c10::cuda::getCurrentCUDAStream(device).stream();
-  const int n_sms = as_int(a.number(23), "n_sms");
+  const int n_sms = a.integer(23, "n_sms");
   int* const status = (int*)a.tensor(24, "status").data_ptr();
   const int out_stride = nh * hd;
   const int *table_p = table.data_ptr<int>(), *cu_p = cu.data_ptr<int>(), *ctx_p = ctx.data_ptr<int>();
@@ -183,7 +196,7 @@ at::Tensor attention(const Args& a) {
     // every sequence brings one token; with sums the scores stay in scratch memory until the rows'
     // maxima and sums are known
     if (T != B) refuse("one token per sequence expected");
-    const int cluster = as_int(a.number(20), "cluster"), groups = as_int(a.number(21), "groups"), n_ctas = as_int(a.number(22), "n_ctas");
+    const int cluster = a.integer(20, "cluster"), groups = a.integer(21, "groups"), n_ctas = a.integer(22, "n_ctas");
     const long pairs = (long)B * nkv;
     at::Tensor part, tickets, scores;
     float *part_o = nullptr, *part_ml = nullptr;
@@ -300,7 +313,7 @@ struct Record {
 
 // select_kept(weight_sums, stored_positions, page_table, stored_lens, next_positions, keep, sinks, recent, status)
 at::Tensor select_kept(const Args& a) {
-  const int keep = as_int(a.number(5), "keep"), sinks = as_int(a.number(6), "sinks"), recent = as_int(a.number(7), "recent");
+  const int keep = a.integer(5, "keep"), sinks = a.integer(6, "sinks"), recent = a.integer(7, "recent");
   const at::Tensor &ws = a.tensor(0, "weight_sums"), &lens = a.tensor(3, "stored_lens"), &next = a.tensor(4, "next_positions");
   const Record r(ws, a.tensor(1, "stored_positions"), a.tensor(2, "page_table"));
   if (!is(lens, at::kInt, r.B, r.device)) refuse("stored_lens must be contiguous int32 [B]");
