@@ -202,3 +202,12 @@ def test_cluster_capacities_are_asked_for_every_device(monkeypatch):
     assert ops.decode_cluster_capacity(128, 4, True) == 11
     device["now"] = 0
     assert ops.decode_cluster_capacity(128, 4, True) == 10 and Library.asked == [0, 1]
+
+
+def test_bounds_of_nothing_are_refused_before_a_plan_is_made():
+    q, i = torch.zeros((1, 64)), torch.zeros(2, dtype=torch.int32)
+    record = dict(weight_sums=torch.zeros(1), stored_positions=i, token_positions=i)
+    for new, ctx in ((1, 0), (0, 64), (1, -5), (-1, 64)):
+        for window, more in ((100, dict(sinks=2)), (None, record)):
+            with pytest.raises(ops.KernelError, match="at least 1"):
+                ops.attention(q, 1, 1, 16, q, q, i, i, i, i, i, 1.0, window, new, ctx, **more)

@@ -768,6 +768,7 @@ def _bounded_attention(q, n_heads, n_kv_heads, head_dim, k_pages, v_pages, page_
     """Attention with a window and sinks, or with sums of weights: the plan of a single-token step is made
     here, checks, memory and launches are csrc/host.cpp's."""
     global launch_count
+    _need(max_ctx_len >= 1 and max_new_tokens >= 1, "max_ctx_len and max_new_tokens must be at least 1")
     if not q.is_cuda:
         raise KernelError("q must be on a CUDA device")
     device = q.get_device()
