@@ -230,3 +230,21 @@ def test_numbers_that_are_none_are_refused():
         with pytest.raises(ops.KernelError, match=name):
             ops.select_kept(sums, stored, table, ints([200]), ints([200]), *numbers)
     assert ops.device_status() == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_scales_that_are_not_positive_are_refused(dtype):
+    """A score that is masked is -inf, which only a positive scale leaves so."""
+    for new in ([1, 1], [30, 1]):
+        s = Step(dtype, 14, 2, 64, [300, 70], new, 100, 4, seed=1)
+        t = Step(dtype, 14, 2, 64, [300, 70], new, seed=1)
+        sums, stored = t.record()
+        for s.scale in (0.0, -0.125, math.nan, math.inf, -math.inf):
+            t.scale = s.scale
+            with pytest.raises(ops.KernelError, match="scale"):
+                s.attend(sinks=4)
+            with pytest.raises(ops.KernelError, match="scale"):
+                t.attend(weight_sums=sums, stored_positions=stored, token_positions=t.pos)
+        s.scale = 1e-6                   # (nearly equal weights)
+        s.check_out(s.attend(sinks=4), s.want())
+    assert ops.device_status() == 0

@@ -148,6 +148,8 @@ at::Tensor attention(const Args& a) {
   const int max_new = a.integer(13, "max_new_tokens"), max_ctx = a.integer(14, "max_ctx_len");
   const bool mma_only = a.number(15, "mma_only") != 0, sums = !a.none(17);
   const int sinks = a.integer(16, "sinks", 1L << 30);
+  // (masked scores are -inf ahead of the scale in some kernels)
+  if (!(scale > 0.f) || scale > 1e30f) refuse("scale must be positive and finite");
   const int device = current_device_of(q, "q");
   const at::ScalarType type = q.scalar_type();
   if (type != at::kBFloat16 && type != at::kFloat) refuse("unsupported element type");
