@@ -248,3 +248,27 @@ def test_scales_that_are_not_positive_are_refused(dtype):
         s.scale = 1e-6                   # (nearly equal weights)
         s.check_out(s.attend(sinks=4), s.want())
     assert ops.device_status() == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("heads", [(14, 2, 64), (28, 4, 128), (4, 2, 48)])
+def test_queries_of_one_row_and_rows_that_overlap(dtype, heads):
+    """One row whose stride says nothing, one row for all tokens, rows that share elements."""
+    nh, nkv, hd = heads
+    for lens, new, strides in (([300], [1], (0, 1, 7, 1 << 40)), ([300, 90], [70, 20], (0, 8, hd)), ([300, 90], [1, 1], (0, 8))):
+        for sums in (False, True):
+            s = Step(dtype, *heads, lens, new, None if sums else 100, 0 if sums else 4, seed=sum(new))
+            T = s.q.shape[0]
+            rows = rnd((nh * hd + T * hd,), dtype, 5)
+            for stride in strides:
+                s.q = rows.as_strided((T, nh * hd), (stride, 1)) if T > 1 else rows[:nh * hd].as_strided((1, nh * hd), (stride, 1))
+                want = s.want()
+                if sums:
+                    old, _ = s.record()
+                    got, stored = s.record()
+                    out = s.attend(weight_sums=got, stored_positions=stored, token_positions=s.pos)
+                    s.check_sums(got, stored, old, want, s.pos)
+                else:
+                    out = s.attend(sinks=4)
+                s.check_out(out, want)
+    assert ops.device_status() == 0

@@ -160,7 +160,8 @@ at::Tensor attention(const Args& a) {
     refuse("pages must be contiguous [n_pages, n_kv_heads, PAGE, head_dim] of q's type, on its device, "
            "and begin at a multiple of 16 bytes");
   const int T = as_int(q.size(0), "the number of tokens"), B = as_int(ctx.numel(), "the number of sequences");
-  const int n_pages = as_int(k.size(0), "n_pages"), q_stride = as_int(q.stride(0), "q's row stride");
+  const int n_pages = as_int(k.size(0), "n_pages");
+  const int q_stride = T == 1 ? nh * hd : as_int(q.stride(0), "q's row stride");     // (a single row's stride may be anything)
   if (table.dim() != 2 || table.size(0) != B) refuse("page_table must have a row for every sequence");
   need_ints(table, "page_table", table.numel(), device);
   need_ints(cu, "cu_seqlens", B + 1L, device);
@@ -233,7 +234,8 @@ at::Tensor attention(const Args& a) {
     lse_p = lse.data_ptr<float>();
   }
   const bool aligned = fast && q_stride % 8 == 0 && address(q) % 16 == 0;      // q rows can be copied 16 bytes at a time
-  const bool on_tc = aligned && !mma_only && wpc_attention_prefill_tc_supports(nh, nkv, hd);
+  // (rows that overlap, an expanded one for instance, cannot be described to the copy engine)
+  const bool on_tc = aligned && !mma_only && q_stride >= nh * hd && wpc_attention_prefill_tc_supports(nh, nkv, hd);
   if (!fast) {
     const int keys = window ? (int)std::min<long>(max_ctx, (long)window + sinks) : max_ctx;
     // Blocks that share a query's keys: about 64 keys each, at most 16, and no more blocks than eight to an SM.
