@@ -272,3 +272,41 @@ def test_queries_of_one_row_and_rows_that_overlap(dtype, heads):
                     out = s.attend(sinks=4)
                 s.check_out(out, want)
     assert ops.device_status() == 0
+
+
+@pytest.mark.parametrize("dtype,heads,how", [
+    (torch.bfloat16, (14, 2, 64), {}), (torch.bfloat16, (14, 2, 64), dict(cluster=0)), (torch.bfloat16, (14, 2, 64), dict(cluster=2)),
+    (torch.bfloat16, (14, 2, 64), dict(cluster=3, groups=2)), (torch.bfloat16, (28, 4, 128), {}), (torch.bfloat16, (28, 4, 128),
+    dict(mma_only=True)), (torch.bfloat16, (4, 2, 48), {}), (torch.float32, (14, 2, 64), {})])
+@pytest.mark.parametrize("sums", [False, True])
+@pytest.mark.parametrize("new", [[1, 1, 1], [40, 1, 30]])
+def test_lengths_beyond_the_page_table_read_nothing_outside_it(dtype, heads, how, sums, new):
+    """The last sequence says that it is longer than its row of the table: it is taken to end there, and the
+    others are right."""
+    s = Step(dtype, *heads, [300, 90, 333], new, None if sums else 100, 0 if sums else 4, seed=6)
+    want = s.want()
+    old, _ = s.record()
+    places = s.table.shape[1] * PAGE
+    s.table[2, -1] = s.spare[0]                                  # (so that its last places exist)
+    first = sum(new[:2])
+    for beyond in (1, 64, 5000):
+        s.ctx[2] = places + beyond
+        s.pos[first:] = torch.arange(places + beyond - new[2], places + beyond, device=DEV)
+        if sums:
+            got, stored = s.record()
+            out = s.attend(weight_sums=got, stored_positions=stored, token_positions=s.pos, **how)
+            mine = {k: w for k, w in want[3].items() if k[0] < 2}
+            pages = sorted({int(p) for p in s.table[:2].flatten().tolist() if p >= 0})
+            expect, bound = old.double().cpu(), torch.zeros_like(old, dtype=torch.float64, device="cpu")
+            for (b, g), w in mine.items():
+                for i in range(s.lens[b]):
+                    page, r = int(s.table[b, i // PAGE]), i % PAGE
+                    before = expect[page, g, r] if i < s.lens[b] - new[b] else torch.zeros(())
+                    bound[page, g, r] = plain.sum_bound(w[i], before, want[2], want[4])
+                    expect[page, g, r] = before + w[i]
+            assert bool(((got.double().cpu() - expect).abs() <= bound)[pages].all())
+        else:
+            out = s.attend(sinks=4, **how)
+        off = (out.double().cpu() - want[0]).abs()[:first]
+        assert bool((off <= plain.out_bound(want[0], want[1], want[2], dtype, 333)[:first]).all())
+    ops.clear_device_status()

@@ -102,6 +102,17 @@ template <int MODE>
 __device__ __forceinline__ int cache_page(const Extra& x, int page) {
   return MODE == MODE_PLAIN ? page : min(page, x.n_pages - 1);     // (negative ones are the loads' own care)
 }
+// A block's place in a row of the page table: its last one for a block beyond it (a length that is too large).
+template <int MODE>
+__device__ __forceinline__ int in_table(int block, int width) {
+  return MODE == MODE_PLAIN ? block : min(block, width - 1);
+}
+// Positions of sequence b, no more than its row of the page table has places for.  (The clusters' decode
+// keeps its look-ups inside the table instead: with this, 8 sequences of 4,001 with their sums took 21.9 us, not 21.5.)
+template <int MODE>
+__device__ __forceinline__ int length_of(const int* ctx_lens, int b, int table_width) {
+  return MODE == MODE_PLAIN ? ctx_lens[b] : min(ctx_lens[b], table_width * WPC_PAGE);
+}
 // The block that number `blk` of a query's range stands for (see the head of this file).
 template <int MODE>
 __device__ __forceinline__ int real_block(int blk, int first, int ns) {
@@ -299,7 +310,7 @@ decode_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, __nv_bfloat16* 
 
   // ---- units of each sequence, and their running sum ----
   for (int b = tid; b < B; b += THREADS) {
-    const int pos = ctx_lens[b] - 1;
+    const int pos = length_of<MODE>(ctx_lens, b, table_width) - 1;
     const int lo = (window > 0 && pos - window + 1 > 0) ? pos - window + 1 : 0;
     s_cum[b + 1] = pos >= 0 ? (pos / PAGE - lo / PAGE + 1 + sink_blocks<MODE>(x, lo / PAGE)) * nkv : 0;
   }
@@ -362,7 +373,7 @@ decode_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, __nv_bfloat16* 
     const int g = within / nb, pg = within - g * nb;
     const int pair_start = s_cum[b] + g * nb, pair_end = pair_start + nb;
     const int seg_end = min(u1, pair_end);
-    const int L = ctx_lens[b];
+    const int L = length_of<MODE>(ctx_lens, b, table_width);
     const int pos = L - 1;
     const int lo = (window > 0 && pos - window + 1 > 0) ? pos - window + 1 : 0;
     const int first = lo / PAGE, ns = sink_blocks<MODE>(x, first);
@@ -637,11 +648,11 @@ decode_cluster_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, __nv_bf
   const int blk0 = g_blk0 + rank * base + min(rank, extra), blk1 = blk0 + base + (rank < extra ? 1 : 0);
   const int* gtable = page_table + (size_t)b * table_width;
   const int n_seg = blk1 - blk0;
-  for (int i = tid; i < min(n_seg, CLUSTER_SEGMENT_PAGES); i += THREADS) s_pages[i] = cache_page<MODE>(x, gtable[real_block<MODE>(blk0 + i, first, ns)]);
+  for (int i = tid; i < min(n_seg, CLUSTER_SEGMENT_PAGES); i += THREADS) s_pages[i] = cache_page<MODE>(x, gtable[in_table<MODE>(real_block<MODE>(blk0 + i, first, ns), table_width)]);
   __syncthreads();                                       // the page numbers are in shared memory for every thread
   auto page_of = [&](int blk) {
     const int i = blk - blk0;
-    return i < CLUSTER_SEGMENT_PAGES ? s_pages[i] : cache_page<MODE>(x, gtable[real_block<MODE>(blk, first, ns)]);
+    return i < CLUSTER_SEGMENT_PAGES ? s_pages[i] : cache_page<MODE>(x, gtable[in_table<MODE>(real_block<MODE>(blk, first, ns), table_width)]);
   };
 
   // The first pages of the ring are started ahead of the dependency wait, except the sequence's
@@ -862,7 +873,7 @@ prefill_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, __nv_bfloat16*
   const int n_rows = n_new * n_rep;
   const int row0 = tile * 64;
   if (row0 >= n_rows) return;                         // whole CTA: no barrier has been used yet
-  const int L = ctx_lens[b];
+  const int L = length_of<MODE>(ctx_lens, b, table_width);
   const int start = L - n_new;                        // position of the sequence's first new token
   const int* table = page_table + (size_t)b * table_width;
   const size_t page_elems = (size_t)nkv * PAGE * HD;

@@ -60,7 +60,7 @@ attention_plain_kernel(const T* __restrict__ q, int q_stride, T* __restrict__ ou
     float m_loc = -INFINITY;
     for (int j = threadIdx.x; j < cn; j += AP_THREADS) {
       const int p = lo + c0 + j + (lo + c0 + j < ns ? 0 : skipped);
-      const int page = min(max(table[p / WPC_PAGE], 0), n_pages - 1);
+      const int page = min(max(table[min(p / WPC_PAGE, table_width - 1)], 0), n_pages - 1);
       const T* kr = k_pages + (((size_t)page * nkv + kvh) * WPC_PAGE + p % WPC_PAGE) * hd;
       float dot = 0.f;
       if ((hd & 3) == 0) {                              // the same order of additions, four elements a load
@@ -99,7 +99,7 @@ attention_plain_kernel(const T* __restrict__ q, int q_stride, T* __restrict__ ou
           const int at = lo + c0 + j, p = at + (at < ns ? 0 : skipped);
           const int in_page = p % WPC_PAGE;
           const int n = min(at < ns ? min(cn - j, ns - at) : cn - j, WPC_PAGE - in_page);
-          const T* vr = v_pages + (((size_t)min(max(table[p / WPC_PAGE], 0), n_pages - 1) * nkv + kvh) * WPC_PAGE + in_page) * hd + d;
+          const T* vr = v_pages + (((size_t)min(max(table[min(p / WPC_PAGE, table_width - 1)], 0), n_pages - 1) * nkv + kvh) * WPC_PAGE + in_page) * hd + d;
           for (int i = 0; i < n; ++i) a = fmaf(ps[j + i], to_float(vr[(size_t)i * hd]), a);
           j += n;
         }

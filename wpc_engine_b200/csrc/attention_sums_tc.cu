@@ -126,10 +126,12 @@ struct SumsWork {
   const int* cu_seqlens;
   const int* ctx_lens;
   int B, nkv, n_rep, key_tiles, tile_tokens;      // key_tiles: of the longest context
+  int places;                                     // that a row of the page table has: no sequence is longer
+  __device__ __forceinline__ int length(int b) const { return min(ctx_lens[b], places); }
 };
 // Query tiles that see a key of tile kt of sequence b.
 __device__ __forceinline__ int query_tiles(const SumsWork& w, int b, int kt) {
-  const int L = w.ctx_lens[b], n_new = w.cu_seqlens[b + 1] - w.cu_seqlens[b];
+  const int L = w.length(b), n_new = w.cu_seqlens[b + 1] - w.cu_seqlens[b];
   if (kt * ST_KEYS >= L || n_new <= 0) return 0;
   return (n_new - max(0, kt * ST_KEYS - (L - n_new)) + w.tile_tokens - 1) / w.tile_tokens;
 }
@@ -144,7 +146,7 @@ struct Segment {
   __device__ __forceinline__ void load(const SumsWork& w) {
     tok0 = w.cu_seqlens[b];
     n_new = w.cu_seqlens[b + 1] - tok0;
-    L = w.ctx_lens[b];
+    L = w.length(b);
     start = L - n_new;
   }
   __device__ __forceinline__ bool next(const SumsWork& w) {
@@ -503,7 +505,7 @@ static int launch_sums(const void* q, int q_stride, int n_tokens, const void* k_
   CUtensorMap mk, mq;
   if (int rc = tc::tensor_map(k_pages, (int)cache_rows, HD, HD, WPC_PAGE, &mk)) return rc;
   if (int rc = tc::tensor_map_heads(q, n_tokens, nh, HD, q_stride, tile_tokens, n_rep, &mq)) return rc;
-  const SumsWork work{cu_seqlens, ctx_lens, B, nkv, n_rep, key_tiles, tile_tokens};
+  const SumsWork work{cu_seqlens, ctx_lens, B, nkv, n_rep, key_tiles, tile_tokens, t.table_width * WPC_PAGE};
   const unsigned ctas = (unsigned)(units < sm_count() ? units : sm_count());
   wpc::launch(prefill_sums_kernel<HD>, dim3(ctas), ST_THREADS, StCfg<HD>::SMEM, stream, mk, mq, work, lse,
               scale * 1.4426950408889634f, t, part, tickets, wait_policy().limit_ns, wait_policy().starve,

@@ -167,7 +167,8 @@ prefill_ws_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
   }
   if (warp == MMA_WARP) tmem_alloc(tmem_holder, W::TMEM_COLS);
 
-  const int L = ctx_lens[b];
+  // (PF_PLAIN takes the caller's word that the page table has a place for every position)
+  const int L = MODE == PF_PLAIN ? ctx_lens[b] : min(ctx_lens[b], table_width * PAGE);
   const int start = L - n_new;
   const int* table = page_table + (size_t)b * table_width;
   // pages that any row of the CTA sees: from the window start of its first row to the position of its last

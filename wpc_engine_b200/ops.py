@@ -676,7 +676,14 @@ def attention(q: torch.Tensor, n_heads: int, n_kv_heads: int, head_dim: int, k_p
     it, and their places in `stored_positions` (int32, the same shape) get `token_positions[t]`
     (int32 [T]).  `positions` are places in the cache here, `token_positions` those in the text:
     they differ once entries have been taken out (`select_kept`).  No page may belong to two
-    sequences of the step."""
+    sequences of the step.
+
+    With sinks or sums, what the cache holds behind a sequence's length may be anything, and so may keys
+    that nobody sees; its values must be finite, since a masked weight of zero times an infinity is none.
+    Page numbers outside the cache and lengths beyond the page table read nothing outside either (the
+    sequence's own result is then worthless).  A step of single tokens starts to copy pages of earlier
+    positions while the kernel ahead of it on the stream still runs: they must have been written before that
+    kernel was queued, or by the kernel directly ahead through `move_kept_` (`set_decode_early_pages`)."""
     sums = weight_sums is not None or stored_positions is not None or token_positions is not None
     if sums:
         if weight_sums is None or stored_positions is None or token_positions is None:
