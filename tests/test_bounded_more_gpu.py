@@ -310,3 +310,68 @@ def test_lengths_beyond_the_page_table_read_nothing_outside_it(dtype, heads, how
         off = (out.double().cpu() - want[0]).abs()[:first]
         assert bool((off <= plain.out_bound(want[0], want[1], want[2], dtype, 333)[:first]).all())
     ops.clear_device_status()
+
+
+def poison():
+    """Fills what the allocator hands out next with NaN, the holes between blocks in use with it; returns the
+    addresses."""
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    blocks = [torch.full((1 << bits,), math.nan, device=DEV)
+              for bits, n in ((20, 16), (19, 32), (18, 64), (16, 128), (14, 256), (12, 512), (10, 1024), (7, 4096)) for _ in range(n)]
+    ranges = [(b.data_ptr(), b.data_ptr() + 4 * b.numel()) for b in blocks]
+    torch.cuda.synchronize()
+    return ranges
+
+
+@pytest.mark.parametrize("heads", [(14, 2, 64), (28, 4, 128), (4, 2, 48)])
+@pytest.mark.parametrize("how", [dict(cluster=0), dict(splits=2), dict(cluster=2), dict(cluster=3, groups=2)])
+@pytest.mark.parametrize("sums", [False, True])
+def test_rows_of_sequences_without_positions_are_written(heads, how, sums):
+    """Outputs and scratch memory come from memory full of NaN."""
+    s = Step(torch.bfloat16, *heads, [300, 64, 90], [1, 1, 1], None if sums else 100, 0 if sums else 5, seed=1)
+    whole = s.want()
+    s.ctx = ints([300, 0, 90])
+    (record, stored), old = s.record(), s.record()[0]
+    ranges = poison()
+    kw = dict(weight_sums=record, stored_positions=stored, token_positions=s.pos) if sums else dict(sinks=5)
+    got = s.attend(**kw, **how)
+    assert any(lo <= got.data_ptr() < hi for lo, hi in ranges)
+    assert bool((got[1] == 0).all())
+    off = (got.double().cpu() - whole[0]).abs()[[0, 2]]
+    assert bool((off <= plain.out_bound(whole[0], whole[1], whole[2], torch.bfloat16, 300)[[0, 2]]).all())
+    if sums:
+        assert torch.equal(record[int(s.table[1, 0])], old[int(s.table[1, 0])]) and bool(record.isfinite().all())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("lens,new", [([300, 70, 129], [300, 70, 129]), ([2300, 90], [40, 2]), ([900, 1, 64], [1, 1, 1])])
+def test_scratch_memory_may_hold_anything(dtype, lens, new):
+    """Sums and sinks over scratch memory full of NaN: whole prompts, shared row tiles, single tokens."""
+    for heads in ((14, 2, 64), (4, 2, 48)):
+        for sums in (False, True):
+            s = Step(dtype, *heads, lens, new, None if sums else 100, 0 if sums else 70, seed=2)
+            want = s.want()
+            old, _ = s.record()
+            record, stored = s.record()
+            ranges = poison()
+            if sums:
+                got = s.attend(weight_sums=record, stored_positions=stored, token_positions=s.pos)
+                s.check_sums(record, stored, old, want, s.pos)
+            else:
+                got = s.attend(sinks=70)
+            assert any(lo <= got.data_ptr() < hi for lo, hi in ranges)
+            s.check_out(got, want)
+
+
+@pytest.mark.parametrize("heads", [(14, 2, 64), (28, 4, 128), (4, 2, 48)])
+def test_keeping_sums_changes_no_bit_of_the_attention(heads):
+    """bfloat16, where both take the same kernel and plan: single tokens, whole prompts, and the mma.sync kernel
+    throughout.  (Row tiles that several CTAs share add up in another order.)"""
+    for lens, new, kws in (([700, 1, 129, 64], [1] * 4, [{}, dict(cluster=0), dict(cluster=2), dict(cluster=3, groups=2)]),
+                           ([1300] * 8, [1300] * 8, [{}, dict(mma_only=True)]), ([700, 300], [40, 2], [dict(mma_only=True)])):
+        s = Step(torch.bfloat16, *heads, lens, new, seed=9)
+        for kw in kws:
+            record, stored = s.record()
+            with_sums = s.attend(weight_sums=record, stored_positions=stored, token_positions=s.pos, **kw)
+            assert torch.equal(with_sums, s.attend(**kw)), (lens, kw)

@@ -682,8 +682,10 @@ def attention(q: torch.Tensor, n_heads: int, n_kv_heads: int, head_dim: int, k_p
     that nobody sees; its values must be finite, since a masked weight of zero times an infinity is none.
     Page numbers outside the cache and lengths beyond the page table read nothing outside either (the
     sequence's own result is then worthless).  A step of single tokens starts to copy pages of earlier
-    positions while the kernel ahead of it on the stream still runs: they must have been written before that
-    kernel was queued, or by the kernel directly ahead through `move_kept_` (`set_decode_early_pages`)."""
+    positions while the kernel ahead of it on the stream still runs: whatever wrote those must be complete when
+    that kernel starts.  `move_kept_` sees to it; behind a kernel of this library that stores earlier positions,
+    a copy or another library's kernel on the stream does (every step of the engine begins with
+    one), or `set_decode_early_pages(False)`."""
     sums = weight_sums is not None or stored_positions is not None or token_positions is not None
     if sums:
         if weight_sums is None or stored_positions is None or token_positions is None:
