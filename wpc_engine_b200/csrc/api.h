@@ -62,11 +62,6 @@ int wpc_gemm_tc_rope_store(const void* w, int ldw, const void* x, int ldx, int t
                            int table_width, const int* seq_of_token, const int* positions, int n_pages, int* status,
                            cudaStream_t stream);
 
-int wpc_attention_plain(const void* q, int q_stride, void* out, int out_stride, int dtype, const void* k_pages,
-                        const void* v_pages, const int* page_table, int table_width, const int* seq_of_token,
-                        const int* positions, int T, int nh, int nkv, int hd, float scale, int window,
-                        int n_splits, float* part, cudaStream_t stream);
-
 // sinks: the first positions that a query sees beside its window (0 without a window);
 // lse: null, or [T][nh] for each row's maximum + log2(sum) of its scores in units of log 2
 int wpc_attention_plain_bounded(const void* q, int q_stride, void* out, int out_stride, int dtype,

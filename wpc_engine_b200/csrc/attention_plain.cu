@@ -166,16 +166,6 @@ __global__ void attention_plain_combine_kernel(const float* __restrict__ part, T
 
 using namespace wpc;
 
-extern "C" int wpc_attention_plain(const void* q, int q_stride, void* out, int out_stride, int dtype,
-                                   const void* k_pages, const void* v_pages, const int* page_table,
-                                   int table_width, const int* seq_of_token, const int* positions, int T, int nh,
-                                   int nkv, int hd, float scale, int window, int n_splits, float* part,
-                                   cudaStream_t stream) {
-  return wpc_attention_plain_bounded(q, q_stride, out, out_stride, dtype, k_pages, v_pages, page_table, table_width,
-                                     seq_of_token, positions, T, nh, nkv, hd, scale, window, 0, n_splits, part, nullptr,
-                                     0x7fffffff, stream);
-}
-
 extern "C" int wpc_attention_plain_bounded(const void* q, int q_stride, void* out, int out_stride, int dtype,
                                            const void* k_pages, const void* v_pages, const int* page_table,
                                            int table_width, const int* seq_of_token, const int* positions, int T,

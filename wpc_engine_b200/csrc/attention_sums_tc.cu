@@ -153,20 +153,17 @@ struct Segment {
     unit += n;
     left -= n;
     if (left <= 0) return false;
-    if (t0 + n < all) { t0 += n; }               // (does not happen: a segment takes all that is left)
-    else {
-      t0 = 0;
-      if (++g == w.nkv) {
-        g = 0;
-        do {
-          if (++kt == w.key_tiles) { kt = 0; ++b; }
-          if (b >= w.B) return false;
-          all = query_tiles(w, b, kt);
-        } while (all == 0);
-        load(w);
-      }
+    t0 = 0;                                      // (a segment takes all that is left of its keys' query tiles)
+    if (++g == w.nkv) {
+      g = 0;
+      do {
+        if (++kt == w.key_tiles) { kt = 0; ++b; }
+        if (b >= w.B) return false;
+        all = query_tiles(w, b, kt);
+      } while (all == 0);
+      load(w);
     }
-    n = min(all - t0, left);
+    n = min(all, left);
     return true;
   }
   __device__ __forceinline__ int key0() const { return kt * ST_KEYS; }
