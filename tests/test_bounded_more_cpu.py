@@ -211,3 +211,6 @@ def test_bounds_of_nothing_are_refused_before_a_plan_is_made():
         for window, more in ((100, dict(sinks=2)), (None, record)):
             with pytest.raises(ops.KernelError, match="at least 1"):
                 ops.attention(q, 1, 1, 16, q, q, i, i, i, i, i, 1.0, window, new, ctx, **more)
+    for new, ctx, name in ((1, 64.0, "max_ctx_len"), ("1", 64, "max_new_tokens"), (None, 64, "max_new_tokens")):
+        with pytest.raises(ops.KernelError, match=name):
+            ops.attention(q, 1, 1, 16, q, q, i, i, i, i, i, 1.0, 100, new, ctx, sinks=2)

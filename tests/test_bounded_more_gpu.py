@@ -375,3 +375,132 @@ def test_keeping_sums_changes_no_bit_of_the_attention(heads):
             record, stored = s.record()
             with_sums = s.attend(weight_sums=record, stored_positions=stored, token_positions=s.pos, **kw)
             assert torch.equal(with_sums, s.attend(**kw)), (lens, kw)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("heads", [(32, 1, 64), (17, 1, 16), (2, 1, 256), (3, 3, 255), (2, 2, 1), (4, 2, 160)])
+@pytest.mark.parametrize("sums", [False, True])
+def test_many_heads_to_a_group_and_head_sizes_of_the_plain_kernels(dtype, heads, sums):
+    for lens, new in (([130, 5, 64], [33, 5, 1]), ([300, 1], [1, 1])):
+        s = Step(dtype, *heads, lens, new, None if sums else 70, 0 if sums else 5, seed=sum(new))
+        want = s.want()
+        if sums:
+            old, _ = s.record()
+            record, stored = s.record()
+            s.check_out(s.attend(weight_sums=record, stored_positions=stored, token_positions=s.pos), want)
+            s.check_sums(record, stored, old, want, s.pos)
+        else:
+            s.check_out(s.attend(sinks=5), want)
+    assert ops.device_status() == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_head_sizes_beyond_the_plain_kernels_are_refused(dtype):
+    for new in ([1, 1], [3, 1]):
+        s = Step(dtype, 2, 1, 260, [70, 5], new, 40, 3, seed=1)
+        with pytest.raises(ops.KernelError, match="unsupported"):
+            s.attend(sinks=3)
+        t = Step(dtype, 2, 1, 260, [70, 5], new, seed=1)
+        record, stored = t.record()
+        with pytest.raises(ops.KernelError, match="unsupported"):
+            t.attend(weight_sums=record, stored_positions=stored, token_positions=t.pos)
+    assert ops.device_status() == 0
+
+
+@pytest.mark.parametrize("heads", [(4, 2, 64), (4, 2, 48)])
+@pytest.mark.parametrize("sums", [False, True])
+def test_a_step_of_more_sequences_than_the_single_token_kernels_take(heads, sums):
+    lens = [1 + 7 * (i % 19) for i in range(1100)]
+    s = Step(torch.bfloat16, *heads, lens, [1] * 1100, None if sums else 40, 0 if sums else 5, seed=3)
+    want = s.want()
+    if sums:
+        old, _ = s.record()
+        record, stored = s.record()
+        s.check_out(s.attend(weight_sums=record, stored_positions=stored, token_positions=s.pos), want)
+        s.check_sums(record, stored, old, want, s.pos)
+    else:
+        s.check_out(s.attend(sinks=5), want)
+    assert ops.device_status() == 0
+
+
+@pytest.mark.parametrize("how", [dict(splits=1), dict(cluster=2), {}])
+def test_shares_of_more_pages_than_their_numbers_are_kept_for(how):
+    """A CTA's share of 625 pages, or 313: page numbers beyond the first 512 or 256 are looked up one by one."""
+    s = Step(torch.bfloat16, 7, 1, 64, [40000], [1], seed=5)
+    old, _ = s.record()
+    record, stored = s.record()
+    full = s.attend(weight_sums=record, stored_positions=stored, token_positions=s.pos, **how)
+    s.check_sums(record, stored, old, fast_want(s), s.pos)
+    w = Step(torch.bfloat16, 7, 1, 64, [40000], [1], 39900, 70, seed=5)
+    x, at = s.q[0, : 7 * 64].double().view(7, 64), torch.arange(40000, device=DEV)
+    pages = s.table[0, at // PAGE].long()
+    k, v = s.k[pages, 0, at % PAGE].double(), s.v[pages, 0, at % PAGE].double()
+    score = x @ k.t() * s.scale
+    err = float((x.abs() @ k.abs().t()).max()) * s.scale * (2 * 64 + 4) * plain.EPS32
+    for got, seen in ((full, at >= 0), (w.attend(sinks=70, **how), (at >= 100) | (at < 70))):
+        p = torch.softmax(score.masked_fill(~seen, -math.inf), 1)
+        bound = plain.out_bound((p @ v), (p @ v.abs()), err, torch.bfloat16, 40000)
+        assert bool(((got.double().view(7, 64) - p @ v).abs() <= bound).all())
+    assert ops.device_status() == 0
+
+
+def alone(script):
+    """Runs the lines in a process of its own, whose arena of tickets is its own too."""
+    import os
+    import subprocess
+    import sys
+    here = os.path.dirname(os.path.abspath(__file__))
+    head = f"""
+import sys
+sys.path[:0] = [{os.path.dirname(here)!r}, {here!r}]
+import torch
+from test_bounded_gpu import Step, ints
+from wpc_engine_b200 import ops
+"""
+    r = subprocess.run([sys.executable, "-c", head + script + "\ntorch.cuda.synchronize()\nprint('ok')"], capture_output=True,
+                       text=True, timeout=300)
+    assert r.returncode == 0 and r.stdout.strip().endswith("ok"), r.stderr[-2000:]
+
+
+def test_captured_calls_beyond_the_arena_of_tickets():
+    """140 captured calls of 8,000 tickets each: the last ones' tickets are zeroed by the graph itself."""
+    alone("""
+lens = [1 + 13 * (i % 30) for i in range(1000)]
+s = Step(torch.bfloat16, 8, 8, 16, lens, [1] * 1000, 100, 5, seed=3)
+want = s.attend(sinks=5, cluster=0)
+graph = torch.cuda.CUDAGraph()
+torch.cuda.synchronize()
+with torch.cuda.graph(graph):
+    outs = [s.attend(sinks=5, cluster=0) for _ in range(140)]
+for _ in range(3):
+    for o in outs:
+        o.fill_(7)
+    graph.replay()
+    assert all(torch.equal(o, want) for o in outs)
+""")
+
+
+def test_a_first_call_that_is_captured():
+    """Nothing was set up outside a capture yet."""
+    alone("""
+ops.host()
+for new, how in (([1] * 8, dict(cluster=0)), ([300] * 8, {})):
+    s = Step(torch.bfloat16, 28, 4, 128, [900] * 8, new, seed=1)
+    sums, stored = s.record()
+    start = sums.clone()
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        out = s.attend(weight_sums=sums, stored_positions=stored, token_positions=s.pos, **how)
+        kept = ops.select_kept(sums, stored, s.table, s.ctx, s.ctx, 100, 4, 30)
+    got = []
+    for _ in range(2):
+        sums.copy_(start)
+        graph.replay()
+        got.append([t.clone() for t in (out, kept, sums)])
+    if new[0] == 300:                    # (eager only at the end: the calls before were the first of all)
+        sums.copy_(start)
+        out = s.attend(weight_sums=sums, stored_positions=stored, token_positions=s.pos, **how)
+        got.append([out, ops.select_kept(sums, stored, s.table, s.ctx, s.ctx, 100, 4, 30), sums])
+    assert all(torch.equal(a, b) for g in got for a, b in zip(g, got[0]))
+""")

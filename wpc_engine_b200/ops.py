@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import operator
 import os
 import threading
 from typing import Optional, Tuple, Union
@@ -134,6 +135,13 @@ def _check(name: str, rc: int) -> None:
 def _need(cond: bool, msg: str) -> None:
     if not cond:
         raise KernelError(msg)
+
+
+def _whole(n, name: str) -> int:
+    try:
+        return operator.index(n)
+    except TypeError:
+        raise KernelError(f"{name} must be a whole number") from None
 
 
 def _rows(t: torch.Tensor, name: str) -> None:
@@ -675,8 +683,8 @@ def attention(q: torch.Tensor, n_heads: int, n_kv_heads: int, head_dim: int, k_p
     group, is added to the entry's place there; the entries of the step's own tokens begin with
     it, and their places in `stored_positions` (int32, the same shape) get `token_positions[t]`
     (int32 [T]).  `positions` are places in the cache here, `token_positions` those in the text:
-    they differ once entries have been taken out (`select_kept`).  No page may belong to two
-    sequences of the step.
+    they differ once entries have been taken out (`select_kept`).  No page may
+    stand twice in the step's page table.
 
     With sinks or sums, what the cache holds behind a sequence's length may be anything, and so may keys
     that nobody sees; its values must be finite, since a masked weight of zero times an infinity is none.
@@ -777,6 +785,7 @@ def _bounded_attention(q, n_heads, n_kv_heads, head_dim, k_pages, v_pages, page_
     """Attention with a window and sinks, or with sums of weights: the plan of a single-token step is made
     here, checks, memory and launches are csrc/host.cpp's."""
     global launch_count
+    max_new_tokens, max_ctx_len = _whole(max_new_tokens, "max_new_tokens"), _whole(max_ctx_len, "max_ctx_len")
     _need(max_ctx_len >= 1 and max_new_tokens >= 1, "max_ctx_len and max_new_tokens must be at least 1")
     if not q.is_cuda:
         raise KernelError("q must be on a CUDA device")
