@@ -1,5 +1,6 @@
 """Operators of bounded caches where several calls meet: after waits that ran out, on several streams, and
 in scratch memory that holds something else."""
+import gc
 import math
 
 import pytest
@@ -315,10 +316,14 @@ def test_lengths_beyond_the_page_table_read_nothing_outside_it(dtype, heads, how
 def poison():
     """Fills what the allocator hands out next with NaN, the holes between blocks in use with it; returns the
     addresses."""
+    gc.collect()
     torch.cuda.synchronize()
     torch.cuda.empty_cache()
-    blocks = [torch.full((1 << bits,), math.nan, device=DEV)
-              for bits, n in ((20, 16), (19, 32), (18, 64), (16, 128), (14, 256), (12, 512), (10, 1024), (7, 4096)) for _ in range(n)]
+    blocks = []
+    for n in [*range(1 << 20, 1 << 18, -(1 << 15)), *(1 << bits for bits in range(18, 6, -1))]:
+        reserved = torch.cuda.memory_reserved()           # (4 MB to 512 bytes, each until no hole of that size is left)
+        while torch.cuda.memory_reserved() == reserved:
+            blocks.append(torch.full((n,), math.nan, device=DEV))
     ranges = [(b.data_ptr(), b.data_ptr() + 4 * b.numel()) for b in blocks]
     torch.cuda.synchronize()
     return ranges
