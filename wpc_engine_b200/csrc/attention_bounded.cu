@@ -9,7 +9,7 @@
 //           row's log-sum of a prefill.
 //
 // Measured (7B shape; 28 heads, 4 KV heads of 128): one sequence at position 24,577, window 4,096, 4 sinks 7.2 us,
-// latency (5 pages a CTA); 64 of up to 8,000, window 2,048, 70 sinks 55.8, 268 MB at 4.8 TB/s; with sums 8
+// latency (5 pages a CTA); 64 of up to 8,000, window 2,048, 70 sinks 55.0 to 58.5, 268 MB at 4.6 to 4.9 TB/s; with sums 8
 // sequences of 4,001 19.5 to 21.7, 67 MB, 17 of it ordinary attention (a second kernel adds up the weights: inside
 // the cluster kernel the same took 24.3), one of 32,768 24.4 to 26.5.
 #include "attention_mma.cuh"

@@ -8,9 +8,10 @@
 // columns, copied to shared memory one tile ahead.  A thread adds the weights of two keys, the
 // four threads that share them add up at the end.  With few keys and many queries the CTAs of a
 // cluster share the queries, every C-th tile each, and rank 0 adds their sums in rank order: the
-// same bits every run.  Bound by the exponentials and the products about equally.  1,000 queries of 4
-// heads of 48 (2 KV heads) over themselves take 32 us, 2,048 behind 3,952 earlier positions 202 us,
-// the attention included.
+// same bits every run.  1,000 queries of 4 heads of 48 (2 KV heads) over themselves take 28 us with
+// the attention, 18 of them without sums; 2,048 behind 3,952 earlier positions 201, this kernel's part 47.  No unit
+// is full there (exponentials 36 %, matrix pipe 19 %): the warps wait for fixed latencies, shared memory and
+// the barriers around a tile, 28 % of them resident.
 #include "attention_mma.cuh"
 #include "attention_sums.cuh"
 

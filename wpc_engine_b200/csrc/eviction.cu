@@ -15,7 +15,8 @@
 //
 // Measured (4 KV heads of 128): the choice of 2,048 of up to 4,096 entries, 28 layers and 8 sequences, 13.0 us (25 MB,
 // 3.8 us at the copy's rate; bound by the counting in shared memory), 44 with the keys read again for each of
-// four digits; one layer of 1,088 entries 4.6, latency.  The moves that follow, 471 MB, 86 us, 5.5 TB/s on rows of
+// four digits; one layer of 1,088 entries 4.6, latency; beyond 32,768 entries 207 us for 20,000 of 40,000, 28 layers,
+// and 312 for 55,000 of 60,000 (loads one behind the other, by one block a row).  The moves that follow, 471 MB, 86 us, 5.5 TB/s on rows of
 // 256 bytes (159 with one row on its way at a time).
 #include "api.h"
 #include "common.cuh"
@@ -393,7 +394,9 @@ int wpc_select_kept(const float* weight_sums, const int* stored_positions, const
   const dim3 grid(nkv, B, layers);
   const size_t layer_stride = (size_t)n_pages * nkv * WPC_PAGE;
   // A thread's share of the keys stays in registers as long as a block of 1,024 threads holds them all
-  // (and the records can be read 16 bytes a load).
+  // (and the records can be read 16 bytes a load): 32,768 entries, 16,384 of which stay, 28 layers 34.6 us, 165
+  // read again for each digit.  Few keys a thread where they fit: 8,192 entries 12.2 us with eight,
+  // 19.2 with thirty-two; 4,096 entries 6.6 with 512 threads, 10.0 with 1,024 (8 sequences: 20.2 and 33.7).
 #define WPC_SELECT(NT, ITEMS)                                                                                        \
   do {                                                                                                               \
     static int configured[MAX_DEVICES];                                                                              \
