@@ -214,3 +214,18 @@ def test_bounds_of_nothing_are_refused_before_a_plan_is_made():
     for new, ctx, name in ((1, 64.0, "max_ctx_len"), ("1", 64, "max_new_tokens"), (None, 64, "max_new_tokens")):
         with pytest.raises(ops.KernelError, match=name):
             ops.attention(q, 1, 1, 16, q, q, i, i, i, i, i, 1.0, 100, new, ctx, sinks=2)
+
+
+def test_parts_of_cache_keep_are_refused_without_it(tmp_path, monkeypatch, capsys):
+    from wpc_engine_b200 import cli
+    wpc.write_random_model(str(tmp_path), wpc.Qwen2Config.from_dict(TINY_A), 1, torch.float32)
+    asked = []
+    monkeypatch.setattr(wpc.Engine, "from_folder", lambda folder, **kw: asked.append(kw["eviction"]) or 1 / 0)
+    run = ["--model", str(tmp_path), "--prompt-ids", "1,2", "--max-tokens", "4"]
+    for flag in ("--cache-recent", "--cache-sinks"):
+        assert cli.main([*run, flag, "0"]) == 2
+        assert f"error: {flag} is a part of --cache-keep" in capsys.readouterr().err
+    for flags, sinks in (([], 4), (["--cache-sinks", "0"], 0), (["--cache-sinks", "9"], 9)):
+        with pytest.raises(ZeroDivisionError):
+            cli.main([*run, "--cache-keep", "64", *flags])
+        assert asked[-1] == CacheEviction(64, 16, sinks)

@@ -52,7 +52,7 @@ def build_parser() -> argparse.ArgumentParser:
                          "a page or two and a step for each sequence")
     ap.add_argument("--cache-recent", type=int, default=None,
                     help="last positions that --cache-keep always holds (default: a quarter of it)")
-    ap.add_argument("--cache-sinks", type=int, default=4, help="first positions that --cache-keep always holds")
+    ap.add_argument("--cache-sinks", type=int, default=None, help="first positions that --cache-keep always holds (default: 4)")
     ap.add_argument("--max-seq-len", type=int, default=None,
                     help="longest sequence (prompt plus generated tokens) that is accepted; default: the model's "
                          "max_position_embeddings")
@@ -92,14 +92,15 @@ def main(argv=None) -> int:
     if args.max_step_tokens is not None and args.max_step_tokens < 1:
         print(f"error: --max-step-tokens must be at least 1, got {args.max_step_tokens}", file=sys.stderr)
         return 2
-    if args.cache_keep is None and args.cache_recent is not None:
-        print("error: --cache-recent is a part of --cache-keep, which is not given", file=sys.stderr)
-        return 2
+    for flag, value in (("--cache-recent", args.cache_recent), ("--cache-sinks", args.cache_sinks)):
+        if args.cache_keep is None and value is not None:
+            print(f"error: {flag} is a part of --cache-keep, which is not given", file=sys.stderr)
+            return 2
     eviction = None
     if args.cache_keep is not None:
         recent = args.cache_keep // 4 if args.cache_recent is None else args.cache_recent
         try:
-            eviction = CacheEviction(args.cache_keep, recent, args.cache_sinks)
+            eviction = CacheEviction(args.cache_keep, recent, 4 if args.cache_sinks is None else args.cache_sinks)
         except ValueError as e:
             print(f"error: {e}", file=sys.stderr)
             return 2
