@@ -216,7 +216,11 @@ class PdlWaiting {
     cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
     unsigned long long id = 0;
     if (cudaGetDevice(&device) != cudaSuccess) device = -1;
-    if (cudaStreamGetCaptureInfo(stream, &status, &id) != cudaSuccess || status == cudaStreamCaptureStatusNone) id = 0;
+    if (cudaStreamGetCaptureInfo(stream, &status, &id) != cudaSuccess) {
+      cudaGetLastError();                                              // (the launch itself will meet what is wrong)
+      id = 0;
+    }
+    if (status == cudaStreamCaptureStatusNone) id = 0;
     return {device, stream, id};
   }
   std::mutex lock_;
