@@ -252,11 +252,11 @@ def test_scales_that_are_not_positive_are_refused(dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
-@pytest.mark.parametrize("heads", [(14, 2, 64), (28, 4, 128), (4, 2, 48)])
+@pytest.mark.parametrize("heads", [(14, 2, 64), (4, 2, 48)])
 def test_queries_of_one_row_and_rows_that_overlap(dtype, heads):
     """One row whose stride says nothing, one row for all tokens, rows that share elements."""
     nh, nkv, hd = heads
-    for lens, new, strides in (([300], [1], (0, 1, 7, 1 << 40)), ([300, 90], [70, 20], (0, 8, hd)), ([300, 90], [1, 1], (0, 8))):
+    for lens, new, strides in (([150], [1], (0, 1, 7, 1 << 40)), ([150, 40], [30, 10], (0, 8, hd)), ([150, 40], [1, 1], (0, 8))):
         for sums in (False, True):
             s = Step(dtype, *heads, lens, new, None if sums else 100, 0 if sums else 4, seed=sum(new))
             T = s.q.shape[0]
@@ -509,3 +509,19 @@ for new, how in (([1] * 8, dict(cluster=0)), ([300] * 8, {})):
         got.append([out, ops.select_kept(sums, stored, s.table, s.ctx, s.ctx, 100, 4, 30), sums])
     assert all(torch.equal(a, b) for g in got for a, b in zip(g, got[0]))
 """)
+
+
+@pytest.mark.parametrize("dtype,heads,new", [(torch.bfloat16, (14, 2, 64), 1), (torch.bfloat16, (14, 2, 64), 30),
+                                             (torch.bfloat16, (4, 2, 48), 30), (torch.float32, (14, 2, 64), 1),
+                                             (torch.float32, (4, 2, 48), 30)])
+def test_sums_of_a_sequence_longer_than_was_stated_are_reported(dtype, heads, new):
+    s = Step(dtype, *heads, [90, 700, 64], [new, new, new], seed=1)
+    for stated, fine in ((100, False), (700, True)):
+        s.max_ctx = stated
+        record, stored = s.record()
+        s.attend(weight_sums=record, stored_positions=stored, token_positions=s.pos)
+        if fine:
+            assert ops.device_status() == 0
+        else:
+            with pytest.raises(ops.KernelError, match="1001"):
+                ops.check_device_status()

@@ -32,7 +32,8 @@ decode_sums_kernel(const float* scores, int score_stride, const float2* row_ml,
   pdl_wait();
   const int g = blockIdx.y, b = blockIdx.z, n_rep = nh / nkv;
   const int key = blockIdx.x * SUMS_THREADS + threadIdx.x;
-  const int L = min(ctx_lens[b], t.table_width * WPC_PAGE);
+  const int stated = ctx_lens[b], L = min(stated, t.table_width * WPC_PAGE);
+  if (key == 0 && g == 0) check_length(t, stated, score_stride);
   if (key >= min(L, score_stride)) return;
   const float* s = scores + ((size_t)(b * nkv + g) * n_rep) * score_stride + key;
   const float2* ml = row_ml + (size_t)b * nh + g * n_rep;
@@ -72,6 +73,7 @@ sums_plain_kernel(const T* q, int q_stride, const T* k_pages, const int* __restr
   const int rank = blockIdx.x % C, blk = blockIdx.x / C, g = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
   const int n_rep = nh / nkv, L = min(ctx_lens[b], t.table_width * WPC_PAGE);
   const int tok0 = cu_seqlens[b], n_new = cu_seqlens[b + 1] - tok0, start = L - n_new;
+  if (blk == 0 && rank == 0 && g == 0 && tid == 0) check_length(t, ctx_lens[b], (int)(gridDim.x / C) * WPC_PAGE);
   if (blk * WPC_PAGE >= L || blk >= t.table_width) return;       // the whole cluster, before any barrier
   if (C > 1) cluster_arrive();
   const int page = min(max(t.page_table[(size_t)b * t.table_width + blk], 0), t.n_pages - 1);

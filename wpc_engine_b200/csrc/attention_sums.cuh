@@ -13,6 +13,12 @@ struct SumsTarget {
   int* status;
 };
 
+// The kernels' grids go by the longest length that the caller stated: a sequence beyond what they cover
+// (`covered` keys) is an error that the host learns of.  For one thread of the sequence.
+__device__ __forceinline__ void check_length(const SumsTarget& t, int length, int covered) {
+  if (length > covered && t.status) atomicExch(t.status, WPC_ERR_BAD_ARGUMENT);
+}
+
 // Adds the sum `w` of key `key` of (sequence b, KV head g); token: the step's token that wrote this
 // key, -1 for a key of an earlier step.
 __device__ __forceinline__ void add_sum(const SumsTarget& t, int nkv, int b, int g, int key, int token, float w) {

@@ -43,6 +43,7 @@ sums_mma_kernel(const __nv_bfloat16* q, int q_stride, const __nv_bfloat16* k_pag
   const int rank = blockIdx.x % C, blk = blockIdx.x / C, g = blockIdx.y, b = blockIdx.z;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int n_rep = nh / nkv, L = min(ctx_lens[b], t.table_width * WPC_PAGE), tok0 = cu_seqlens[b], n_new = cu_seqlens[b + 1] - tok0, start = L - n_new;
+  if (blk == 0 && rank == 0 && g == 0 && tid == 0) check_length(t, ctx_lens[b], (int)(gridDim.x / C) * PAGE);
   if (blk * PAGE >= L || blk >= t.table_width || n_new <= 0) return;      // the whole cluster, before any barrier
   if (C > 1) cluster_arrive();
   const int page = min(max(t.page_table[(size_t)b * t.table_width + blk], 0), t.n_pages - 1);

@@ -388,6 +388,7 @@ prefill_sums_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     int filled = 0;                                          // units of this half so far
     bool ok = true, more = true;
     while (more) {
+      if (tid == 0 && sg.kt == 0 && sg.t0 == 0 && sg.g == 0) check_length(t, work.ctx_lens[sg.b], work.key_tiles * ST_KEYS);
       const int key = sg.key0() + half * 128 + r;
       const int i0 = sg.first_of(work, half);
       int tile_first = sg.token(work, i0);                   // first token of the next query tile

@@ -23,7 +23,8 @@ _F32, _BF16 = 0, 1
 _ERRORS = {1001: "bad argument", 1002: "unsupported size", 1003: "size beyond the stated maximum",
            1004: "a device-side wait ran out"}
 # what a non-zero device status word means (written by kernels, read by the host after them)
-_DEVICE_ERRORS = {1001: "a token's position has no page in the cache (its key and value were not written)",
+_DEVICE_ERRORS = {1001: "a token's position has no page in the cache (its key and value were not written), or a length is beyond "
+                        "what the caller stated",
                   1004: "a wait inside a kernel ran out; the kernel returned without finishing its output"}
 
 
@@ -673,6 +674,9 @@ def attention(q: torch.Tensor, n_heads: int, n_kv_heads: int, head_dim: int, k_p
     about that many CTAs to a pair, `cluster` `groups` clusters of that size to a pair, 0 none); otherwise the
     tcgen05 kernel for head sizes 64 and 128 (csrc/attention_tc.cu) and the mma.sync kernel for
     the others (or with `mma_only`).  Everything else runs the plain kernel.
+
+    `max_new_tokens` and `max_ctx_len`: no sequence of the step brings more tokens or is longer afterwards (grids and
+    plans go by them; a sequence whose sums they do not cover sets the device error word, 1001).
 
     `sinks`: beside its window a query sees the first `sinks` positions (their pages must be in the
     page table; pages between the sinks and the window may be gone).  Without a window it
