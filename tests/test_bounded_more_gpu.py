@@ -329,8 +329,8 @@ def poison():
     return ranges
 
 
-@pytest.mark.parametrize("heads", [(14, 2, 64), (28, 4, 128), (4, 2, 48)])
-@pytest.mark.parametrize("how", [dict(cluster=0), dict(splits=2), dict(cluster=2), dict(cluster=3, groups=2)])
+@pytest.mark.parametrize("heads", [(14, 2, 64), (4, 2, 48)])
+@pytest.mark.parametrize("how", [dict(cluster=0), dict(cluster=2), dict(cluster=3, groups=2)])
 @pytest.mark.parametrize("sums", [False, True])
 def test_rows_of_sequences_without_positions_are_written(heads, how, sums):
     """Outputs and scratch memory come from memory full of NaN."""
@@ -350,23 +350,22 @@ def test_rows_of_sequences_without_positions_are_written(heads, how, sums):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
-@pytest.mark.parametrize("lens,new", [([300, 70, 129], [300, 70, 129]), ([2300, 90], [40, 2]), ([900, 1, 64], [1, 1, 1])])
+@pytest.mark.parametrize("lens,new", [([150, 70, 129], [150, 70, 129]), ([2300, 90], [40, 2]), ([900, 1, 64], [1, 1, 1])])
 def test_scratch_memory_may_hold_anything(dtype, lens, new):
     """Sums and sinks over scratch memory full of NaN: whole prompts, shared row tiles, single tokens."""
-    for heads in ((14, 2, 64), (4, 2, 48)):
-        for sums in (False, True):
-            s = Step(dtype, *heads, lens, new, None if sums else 100, 0 if sums else 70, seed=2)
-            want = s.want()
-            old, _ = s.record()
-            record, stored = s.record()
-            ranges = poison()
-            if sums:
-                got = s.attend(weight_sums=record, stored_positions=stored, token_positions=s.pos)
-                s.check_sums(record, stored, old, want, s.pos)
-            else:
-                got = s.attend(sinks=70)
-            assert any(lo <= got.data_ptr() < hi for lo, hi in ranges)
-            s.check_out(got, want)
+    for heads, sums in (((14, 2, 64), False), ((14, 2, 64), True), ((4, 2, 48), True)):
+        s = Step(dtype, *heads, lens, new, None if sums else 100, 0 if sums else 70, seed=2)
+        want = s.want()
+        old, _ = s.record()
+        record, stored = s.record()
+        ranges = poison()
+        if sums:
+            got = s.attend(weight_sums=record, stored_positions=stored, token_positions=s.pos)
+            s.check_sums(record, stored, old, want, s.pos)
+        else:
+            got = s.attend(sinks=70)
+        assert any(lo <= got.data_ptr() < hi for lo, hi in ranges)
+        s.check_out(got, want)
 
 
 @pytest.mark.parametrize("heads", [(14, 2, 64), (28, 4, 128), (4, 2, 48)])
