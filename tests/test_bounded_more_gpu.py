@@ -524,3 +524,47 @@ def test_sums_of_a_sequence_longer_than_was_stated_are_reported(dtype, heads, ne
         else:
             with pytest.raises(ops.KernelError, match="1001"):
                 ops.check_device_status()
+
+
+@pytest.mark.parametrize("heads", [(14, 2, 64), (28, 4, 128), (4, 2, 48)])
+def test_prompts_on_two_streams_at_once(heads):
+    """Sums of prompts, of chunks over a long cache, the choice and the moves on two streams, an eager one and
+    one that replays a graph: no scratch memory, no tickets and no results are shared."""
+    steps = [Step(torch.bfloat16, *heads, [700, 300], [700, 300], seed=1), Step(torch.bfloat16, *heads, [2300, 1000], [40, 30], seed=2)]
+    lens = [ints([n] * len(s.lens)) for s, n in zip(steps, (300, 900))]
+
+    def run(i):
+        s = steps[i]
+        sums, stored = records[i]
+        out = s.attend(weight_sums=sums, stored_positions=stored, token_positions=s.pos)
+        kept = ops.select_kept(sums, stored, s.table, lens[i], s.ctx, 128, 4, 30)
+        ops.move_kept_(s.k, s.v, sums, stored, s.table, kept)
+        return out, kept, s.k, s.v, sums, stored
+
+    records = [s.record() for s in steps]
+    start = [[t.clone() for t in (s.k, s.v, *r)] for s, r in zip(steps, records)]
+
+    def reset(i):
+        for t, o in zip((steps[i].k, steps[i].v, *records[i]), start[i]):
+            t.copy_(o)
+
+    want = []
+    for i in range(2):
+        want.append([t.clone() for t in run(i)])
+        reset(i)
+    graph, streams = torch.cuda.CUDAGraph(), [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        captured = run(1)
+    for _ in range(10):
+        for i in range(2):
+            reset(i)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(streams[0]):
+            got = run(0)
+        with torch.cuda.stream(streams[1]):
+            graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want[0]))
+        assert all(torch.equal(a, b) for a, b in zip(captured, want[1]))
+    assert ops.device_status() == 0

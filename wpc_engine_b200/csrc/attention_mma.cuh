@@ -226,6 +226,9 @@ __device__ __forceinline__ void softmax_step(float (&s)[NT][4], float (&m)[2], f
   }
 }
 
+// The weights as the second product's operand: rounded to the values' type, since a matrix instruction takes
+// both operands in one type (at most half a step, 2^-8 of a weight, as the rounding of the output; two
+// bfloat16 a weight would double the product).  Sums of weights and the denominators use them unrounded.
 template <int NT>
 __device__ __forceinline__ void to_fragments(const float (&s)[NT][4], uint32_t (&pf)[NT / 2][4]) {
 #pragma unroll

@@ -13,6 +13,8 @@
 //                  [64, hd] as it lies in the cache (hd contiguous: an MN-major B operand),
 //                  O [128, hd] float32 in tensor memory
 //
+// P is rounded to the values' type, since a matrix instruction takes both operands in one type (at most half a step, 2^-8 of
+// a weight, as the rounding of the output); its sums are those of the unrounded weights.
 // The running maximum that the exponentials use is only raised when the true maximum has
 // grown by more than 8 (a factor 256, harmless in float32); then the thread rescales its row
 // of O in tensor memory.  Separate warps copy the pages (TMA), issue the MMAs and do the
