@@ -229,3 +229,23 @@ def test_parts_of_cache_keep_are_refused_without_it(tmp_path, monkeypatch, capsy
         with pytest.raises(ZeroDivisionError):
             cli.main([*run, "--cache-keep", "64", *flags])
         assert asked[-1] == CacheEviction(64, 16, sinks)
+
+
+def test_a_layer_cannot_see_more_sinks_than_the_cache_that_it_reads_keeps():
+    from wpc_engine_b200.models import DecoderModel, Run
+    from wpc_engine_b200.registry import resolve
+    cfg = wpc.Qwen2Config.from_dict(dict(TINY_C, attention_sinks=5))            # layers 1 and 2: window 40, 5 sinks
+    base = resolve(cfg.to_dict()).build(cfg)
+
+    def build(kept, seen, reads=2):
+        base.blocks[1].mixer.sinks, base.blocks[2].mixer.sinks = kept, seen
+        return DecoderModel(cfg, base.embedding, base.blocks, base.final_norm, base.head,
+                            schedule=[Run(0), Run(1), Run(reads, cache_of=1 if reads == 2 else 0)])
+    for kept, seen in ((5, 5), (5, 0), (0, 0), (5, 4)):
+        build(kept, seen)
+    for kept, seen in ((0, 1), (4, 5)):
+        with pytest.raises(ValueError, match="sinks"):
+            build(kept, seen)
+    build(0, 0, reads=1)                                                          # (layer 0 keeps everything)
+    base.blocks[1].mixer.sinks = 5
+    DecoderModel(cfg, base.embedding, base.blocks, base.final_norm, base.head, schedule=[Run(0), Run(1, cache_of=0)])

@@ -54,6 +54,16 @@ class DecoderModel:
                 if not 0 <= run.cache_of < i or self.schedule[run.cache_of].cache_of is not None:
                     raise ValueError(f"schedule entry {i} reads the cache of entry {run.cache_of}, "
                                      "which is not an earlier entry with a cache of its own")
+                self._check_sinks(i, run)
+
+    def _check_sinks(self, i: int, run: Run) -> None:
+        """A cache with a window gives the pages between its own sinks and the window back: a layer that reads
+        it cannot see more sinks than it keeps."""
+        own, kept = (None if m is None else m.cache_spec() for m in
+                     (self.blocks[run.layer].mixer_of(), self.blocks[self.schedule[run.cache_of].layer].mixer_of()))
+        if isinstance(own, KVSpec) and isinstance(kept, KVSpec) and kept.window is not None and own.sinks > kept.sinks:
+            raise ValueError(f"schedule entry {i} sees {own.sinks} sinks, but the cache of entry {run.cache_of} keeps "
+                             f"{kept.sinks} beside its window")
 
     @property
     def vocab_size(self) -> int:
