@@ -568,3 +568,30 @@ def test_prompts_on_two_streams_at_once(heads):
         assert all(torch.equal(a, b) for a, b in zip(got, want[0]))
         assert all(torch.equal(a, b) for a, b in zip(captured, want[1]))
     assert ops.device_status() == 0
+
+
+@pytest.mark.parametrize("heads", [(14, 2, 64), (28, 4, 128)])
+@pytest.mark.parametrize("lens,new", [([90] * 150, [3] * 150), ([2300, 700], [20, 30])])
+def test_attention_that_gave_up_does_no_harm_to_the_sums_of_earlier_entries(heads, lens, new):
+    """The attention starves everywhere and leaves no log-sums; half of the CTAs of the sums work with what it
+    left, from memory full of NaN: whole row tiles, and shared ones."""
+    s = Step(torch.bfloat16, *heads, lens, new, seed=1)
+    old, _ = s.record()
+    for starve in (2, 1):
+        record, stored = s.record()
+        ranges = poison()
+        try:
+            ops.set_wait_policy(2_000_000, starve=starve)
+            out = s.attend(weight_sums=record, stored_positions=stored, token_positions=s.pos)
+            torch.cuda.synchronize()
+        finally:
+            ops.set_wait_policy()
+        assert any(lo <= out.data_ptr() < hi for lo, hi in ranges)
+        with pytest.raises(ops.KernelError, match="1004"):
+            ops.check_device_status()
+        table = s.table.tolist()
+        for b, (n, m) in enumerate(zip(lens, new)):
+            at = torch.arange(n - m)
+            pages = torch.tensor([table[b][i // PAGE] for i in at.tolist()])
+            assert torch.equal(record.cpu()[pages, :, at % PAGE], old.cpu()[pages, :, at % PAGE])
+    assert ops.device_status() == 0

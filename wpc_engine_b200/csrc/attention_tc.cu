@@ -420,7 +420,7 @@ prefill_ws_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     if constexpr (SHARED) {
       // slot [HD / 4][128 rows] of four values: neighbouring rows lie side by side
       const size_t slot = ((size_t)blockIdx.z * gridDim.y + tile) * gridDim.x + g;
-      if (valid) part_ml[slot * ROWS + rt] = make_float2(m_used, l_sum);
+      if (valid) part_ml[slot * ROWS + rt] = make_float2(m_used, ok ? l_sum : -1.f);      // (-1: a wait ran out)
       if (ok && n_pg > 0) {
 #pragma unroll
         for (int c = 0; c < HD; c += 32) {
@@ -456,6 +456,9 @@ prefill_ws_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
           }
         }
       }
+    } else if ((MODE & PF_SUMS) && valid) {
+      // (a wait ran out: the row's weights count as nothing, so the sums of earlier entries take no harm)
+      lse[(size_t)(tok0 + t_row) * nh + h_row] = INFINITY;
     }
   }
   fence_before_sync();
@@ -493,6 +496,7 @@ prefill_join_kernel(const float4* part_o, const float2* part_ml, __nv_bfloat16* 
 #pragma unroll 4
   for (int s = 0; s < n_splits; ++s) m = fmaxf(m, part_ml[slot(s) * ROWS + rt].x);
   float den = 0.f, num[JOIN] = {};
+  bool lost = false;
   for (int s0 = 0; s0 < n_splits; s0 += 4) {               // (four shares' loads on their way at once)
     float2 ml[4];
     float4 o[4][JOIN / 4];
@@ -505,6 +509,7 @@ prefill_join_kernel(const float4* part_o, const float2* part_ml, __nv_bfloat16* 
         o[k][i] = ml[k].y != 0.f ? part_o[(slot(s0 + k) * (HD / 4) + part * (JOIN / 4) + i) * ROWS + rt] : make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
+      lost |= ml[k].y < 0.f;
       const float f = ml[k].y != 0.f ? exp2f(ml[k].x - m) : 0.f;
       den = fmaf(f, ml[k].y, den);
 #pragma unroll
@@ -527,7 +532,7 @@ prefill_join_kernel(const float4* part_o, const float2* part_ml, __nv_bfloat16* 
   uint4* dst = (uint4*)(out + (size_t)tok * out_stride + (size_t)h * HD + part * JOIN);
 #pragma unroll
   for (int i = 0; i < JOIN / 8; ++i) dst[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
-  if (lse && part == 0) lse[(size_t)tok * nh + h] = m + log2f(den);
+  if (lse && part == 0) lse[(size_t)tok * nh + h] = lost ? INFINITY : m + log2f(den);
 }
 
 template <int HD, int NT, int MODE = PF_PLAIN>

@@ -191,7 +191,7 @@ class Engine:
         step, which waits for the device, and raise `KernelError` if a kernel of the step gave
         up.  A step that raises, for whatever reason, leaves the sequences as they were: the
         pages that it had taken go back.  (With eviction a step that a kernel gave up in may have added
-        to the sums of entries stored before it.)
+        weights of the queries that it did serve to the sums of entries stored before it.)
 
         With eviction, sequences that hold too many entries afterwards are cut down to what is kept.  If
         that cannot be done (no memory for the choice), the step still counts and its logits are
