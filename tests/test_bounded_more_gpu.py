@@ -595,3 +595,24 @@ def test_attention_that_gave_up_does_no_harm_to_the_sums_of_earlier_entries(head
             pages = torch.tensor([table[b][i // PAGE] for i in at.tolist()])
             assert torch.equal(record.cpu()[pages, :, at % PAGE], old.cpu()[pages, :, at % PAGE])
     assert ops.device_status() == 0
+
+
+def test_a_launch_that_fails_does_not_use_up_the_wait():
+    """70,000 sequences are more than a grid has layers: the launch is refused, and the kernel behind the move is
+    still the next one."""
+    move, _ = a_move()
+    B = 70000
+    q, one = torch.zeros((B, 96), dtype=torch.bfloat16, device=DEV), torch.ones(B, dtype=torch.int32, device=DEV)
+    pages, table = torch.zeros((1, 2, PAGE, 48), dtype=torch.bfloat16, device=DEV), torch.zeros((B, 1), dtype=torch.int32, device=DEV)
+    seq = torch.arange(B + 1, dtype=torch.int32, device=DEV)
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        move()
+        with pytest.raises(ops.KernelError):
+            ops.attention(q, 2, 2, 48, pages, pages, table, seq, one, seq[:B], one - 1, 1.0, 10, 1, 1, sinks=1)
+        assert waits(stream)
+        ops.rmsnorm(torch.ones(4, 64, device=DEV), torch.ones(64, device=DEV), 1e-6, torch.float32)
+        assert not waits(stream)
+    torch.cuda.synchronize()
+    assert ops.device_status() == 0

@@ -123,7 +123,8 @@ def main(argv=None) -> int:
         need = max((len(p) + args.max_tokens + PAGE - 1) // PAGE * PAGE for p in prompts) * args.max_batch
     # (as many sequences as can be alive at once: what bounds a sequence's pages then bounds the cache)
     engine = Engine.from_folder(args.model, dtype=dtype, device="cuda", max_tokens=args.cache_tokens or need,
-                                max_sequences=min(len(prompts), args.max_batch or len(prompts)), max_step_tokens=args.max_step_tokens, eviction=eviction)
+                                max_sequences=min(len(prompts), args.max_batch or len(prompts)),
+                                max_step_tokens=args.max_step_tokens, eviction=eviction)
     c = engine.config
     print(f"config: hidden={c.hidden_size} layers={c.num_hidden_layers} heads={c.num_attention_heads} "
           f"kv_heads={c.num_key_value_heads} vocab={c.vocab_size}", file=sys.stderr)

@@ -192,17 +192,19 @@ class PdlWaiting {
     queues_.insert(q);
     n_.store((int)queues_.size(), std::memory_order_release);
   }
-  // Whether the next kernel of `stream` has to wait; take: it is being launched.
-  bool next(cudaStream_t stream, bool take) {
+  // Whether the next kernel of `stream` has to wait.
+  bool next(cudaStream_t stream) {
     if (n_.load(std::memory_order_acquire) == 0) return false;         // (every launch asks)
     const Queue q = queue(stream);
     std::lock_guard<std::mutex> hold(lock_);
-    const bool waits = queues_.count(q) != 0;
-    if (waits && take) {
-      queues_.erase(q);
-      n_.store((int)queues_.size(), std::memory_order_release);
-    }
-    return waits;
+    return queues_.count(q) != 0;
+  }
+  // That kernel has been launched.
+  void done(cudaStream_t stream) {
+    const Queue q = queue(stream);
+    std::lock_guard<std::mutex> hold(lock_);
+    queues_.erase(q);
+    n_.store((int)queues_.size(), std::memory_order_release);
   }
   static PdlWaiting& all() {
     static auto* w = new PdlWaiting();                                 // (outlives the process's last launch)
@@ -227,14 +229,14 @@ class PdlWaiting {
   std::set<Queue> queues_;
   std::atomic<int> n_{0};
 };
-inline bool pdl_allowed(cudaStream_t stream) {
-  const bool waits = PdlWaiting::all().next(stream, true), skip = pdl_skip_next() != 0;
-  pdl_skip_next() = 0;
-  return pdl_enabled() && !waits && !skip;
-}
 inline int& last_launch_error() {
   static thread_local int rc = 0;
   return rc;
+}
+inline void launched(cudaError_t e, bool waits, cudaStream_t stream) {
+  pdl_skip_next() = 0;
+  if (e != cudaSuccess) last_launch_error() = (int)e;
+  else if (waits) PdlWaiting::all().done(stream);
 }
 
 template <typename... KArgs, typename... Args>
@@ -248,9 +250,9 @@ inline void launch(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem,
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = pdl_allowed(stream) ? 1 : 0;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
-  if (e != cudaSuccess) last_launch_error() = (int)e;
+  const bool waits = PdlWaiting::all().next(stream);
+  cfg.numAttrs = pdl_enabled() && !waits && !pdl_skip_next() ? 1 : 0;
+  launched(cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...), waits, stream);
 }
 
 // The same with thread-block clusters of `cluster_x` CTAs along x (gridDim.x a multiple of it).
@@ -270,9 +272,9 @@ inline void launch_clusters(void (*kernel)(KArgs...), dim3 grid, dim3 block, siz
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = pdl_allowed(stream) ? 2 : 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
-  if (e != cudaSuccess) last_launch_error() = (int)e;
+  const bool waits = PdlWaiting::all().next(stream);
+  cfg.numAttrs = pdl_enabled() && !waits && !pdl_skip_next() ? 2 : 1;
+  launched(cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...), waits, stream);
 }
 
 // ---- bounded waits ------------------------------------------------------------------------------

@@ -336,7 +336,7 @@ int wpc_set_pdl(int on) {
   return was;
 }
 
-int wpc_pdl_next_waits(cudaStream_t stream) { return PdlWaiting::all().next(stream, false) ? 1 : 0; }
+int wpc_pdl_next_waits(cudaStream_t stream) { return PdlWaiting::all().next(stream) ? 1 : 0; }
 
 int wpc_set_wait_policy(unsigned long long limit_ns, int starve) {
   if (limit_ns == 0 || starve < 0 || starve > STARVE_ODD) return WPC_ERR_BAD_ARGUMENT;
