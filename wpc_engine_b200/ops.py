@@ -690,7 +690,7 @@ def attention(q: torch.Tensor, n_heads: int, n_kv_heads: int, head_dim: int, k_p
     they differ once entries have been taken out (`select_kept`).  No page may
     stand twice in the step's page table.
 
-    With sinks or sums, what the cache holds behind a sequence's length may be anything, and so may keys
+    With sinks or sums, `scale` must be positive.  What the cache holds behind a sequence's length may be anything, and so may keys
     that nobody sees; its values must be finite, since a masked weight of zero times an infinity is none.
     Page numbers outside the cache and lengths beyond the page table read nothing outside either (the
     sequence's own result is then worthless).  A step of single tokens starts to copy pages of earlier
