@@ -9,9 +9,11 @@
 // four threads that share them add up at the end.  With few keys and many queries the CTAs of a
 // cluster share the queries, every C-th tile each, and rank 0 adds their sums in rank order: the
 // same bits every run.  1,000 queries of 4 heads of 48 (2 KV heads) over themselves take 28 us with
-// the attention, 18 of them without sums; 2,048 behind 3,952 earlier positions 201, this kernel's part 47.  No unit
-// is full there (exponentials 36 %, matrix pipe 19 %): the warps wait for fixed latencies, shared memory and
-// the barriers around a tile, 28 % of them resident.
+// the attention, 18 of them without sums; 2,048 behind 3,952 earlier positions 201, 102 of them without.
+// Alone this kernel takes 47 there, no unit full (exponentials 36 %, matrix pipe 19 %; the warps wait for fixed
+// latencies, shared memory and the barriers around a tile); behind the attention its CTAs become
+// resident early, crowded on the SMs that the attention leaves free, and take twice as long (136 in all
+// without early starts anywhere).
 #include "attention_mma.cuh"
 #include "attention_sums.cuh"
 
